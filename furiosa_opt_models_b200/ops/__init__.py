@@ -6,6 +6,12 @@ GPU host raises, so no test or benchmark silently runs a PyTorch fallback.
 """
 
 from .native import native, scratch  # noqa: F401
+from .decode import (  # noqa: F401
+    QuantizedCache,
+    paged_tree,
+    process_logits,
+    tree_mask,
+)
 from .kernels import (  # noqa: F401
     EPI_BF16,
     EPI_F32,

@@ -6,6 +6,7 @@ from dataclasses import dataclass
 
 import torch
 
+from .decode import QuantizedCache, paged_tree, store_rows
 from .native import native, scratch
 
 EPI_BF16, EPI_F32, EPI_SWIGLU = 0, 1, 2
@@ -271,7 +272,20 @@ def argmax(logits: torch.Tensor, valid: int | None = None, base: int = 0):
 
 
 def qk_norm_rope_cache(qkv, q_heads, kv_heads, head_dim, q_norm, k_norm, eps, positions, inv_freq,
-                       attention_factor, cache, slots):
+                       attention_factor, cache, slots, rotary_dim=None, interleaved=False):
+    """Per-head norm (weights or None) and rotation of packed q/k/v rows; returns q [rows, q_heads, d]
+    and writes the k and v rows to their cache slots (a negative slot: not cached).
+
+    The rotation turns the pairs (j, j + r / 2) of a head's first r = ``rotary_dim`` elements (all by
+    default), or (2j, 2j + 1) with ``interleaved``, by position * inv_freq[j], cos and sin times
+    ``attention_factor``. Over a ``QuantizedCache``, or with a partial or interleaved rotation, the
+    angle is formed in 64 bits and the normed row stays FP32 until it is stored; over BF16 pages with
+    the full half-split rotation the angle is FP32 and the norm's output rounds to BF16 first, as the
+    decoders run it. The slots of a call that are not negative are distinct: what a slot named by two
+    rows holds is unspecified."""
+    if isinstance(cache, QuantizedCache) or interleaved or rotary_dim not in (None, head_dim):
+        return store_rows(qkv, q_heads, kv_heads, head_dim, q_norm, k_norm, eps, positions, inv_freq,
+                          attention_factor, cache, slots, rotary_dim, interleaved)
     rows = qkv.shape[0]
     q = torch.empty(rows, q_heads, head_dim, dtype=torch.bfloat16, device=qkv.device)
     native().ops.qk_norm_rope_cache(
@@ -287,13 +301,20 @@ def _attn_common(segments: torch.Tensor) -> None:
         raise ValueError("segments are int32 [n, 5]: row_start, len, cached, table_start, nblocks")
 
 
-def paged_decode(q, cache, table, segments, kv_heads, max_keys, scale=None, keys_per_split=2048, out=None,
+def paged_decode(q, cache, table, segments, kv_heads, max_keys, scale=None, keys_per_split=None, out=None,
                  counters=None, warps=0, stages=0):
     """Flash-decoding of one-row segments over the paged cache. q: [rows, q_heads, d]. With
     `counters` (int32, zero, one per segment and key/value head) the splits merge in the kernel.
     `warps` (2-4) and `stages` (2-3) pick the CTA shape (0: the engine's defaults); measurements
-    compare them."""
+    compare them. `keys_per_split` is 2048 over BF16 pages; over a ``QuantizedCache`` (which takes
+    none of counters, warps and stages) it follows the call's sizes as in ``paged_tree``."""
     _attn_common(segments)
+    if isinstance(cache, QuantizedCache):
+        if counters is not None or warps or stages:
+            raise ValueError("counters, warps and stages are of BF16 pages")
+        return paged_tree(q, cache, table, segments, kv_heads, max_keys, 1, scale=scale, keys_per_split=keys_per_split,
+                          out=out)
+    keys_per_split = 2048 if keys_per_split is None else keys_per_split
     rows, q_heads, d = q.shape
     out = torch.empty_like(q) if out is None else out
     s = scratch(q.device)
@@ -329,6 +350,8 @@ def paged_prefill(q, cache, table, segments, kv_heads, work, scale=None, out=Non
     of its segment, as encoders do). ``cache`` is the layer's pages [blocks, 2, kv_heads, 16, d];
     ``tensor_cores=False`` runs the mma.sync kernel."""
     _attn_common(segments)
+    if isinstance(cache, QuantizedCache):
+        raise ValueError("paged_prefill reads BF16 pages: paged_tree attends chunks over a QuantizedCache")
     rows, q_heads, d = q.shape
     out = torch.empty_like(q) if out is None else out
     s = scratch(q.device)

@@ -1,0 +1,147 @@
+"""Decode-step operators on the host: drafted-tree masks, the quantized cache's views, refusals."""
+
+import pytest
+import torch
+
+from furiosa_opt_models_b200 import ops
+
+BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
+
+
+def test_tree_mask_holds_ancestors_and_the_node_itself():
+    # 0 - 1 - 3, 0 - 2, and 4 a second root; a chain of 40 in the second segment (two words).
+    mask = ops.tree_mask([[-1, 0, 0, 1, -1], [i - 1 for i in range(40)]])
+    assert mask.shape == (45, 2) and mask.dtype == I32
+    bits = [[j for j in range(64) if mask[r, j // 32].item() >> (j % 32) & 1] for r in range(45)]
+    assert bits[:5] == [[0], [0, 1], [0, 2], [0, 1, 3], [4]]
+    assert bits[5:] == [list(range(i + 1)) for i in range(40)]
+    assert ops.tree_mask([]).shape == (0, 1)
+    assert ops.tree_mask([[], [-1]]).tolist() == [[1]]
+
+
+@pytest.mark.parametrize("parents", [[[0]], [[-1, 1]], [[-1, 2, 0]], [[-2]]])
+def test_tree_mask_refuses_parents_that_do_not_come_before(parents):
+    with pytest.raises(ValueError, match="parents come before"):
+        ops.tree_mask(parents)
+
+
+def test_quantized_cache_views():
+    c = ops.QuantizedCache.empty(3, 2, 64, device="cpu")
+    assert c.pages.shape == (3, 2, 2, 16 * 64 + 64)
+    assert c.codes.shape == (3, 2, 2, 16, 64) and c.scales.shape == (3, 2, 2, 16)
+    assert torch.count_nonzero(c.dequantize()) == 0
+    c.codes[1, 0, 1, 5] = torch.full((64,), 1.5).to(torch.float8_e4m3fn).view(torch.uint8)
+    c.scales[1, 0, 1, 5] = 0.25
+    v = c.dequantize()
+    assert torch.equal(v[1, 0, 1, 5], torch.full((64,), 0.375)) and torch.count_nonzero(v) == 64
+
+
+@pytest.mark.parametrize("pages,d", [
+    (torch.zeros(2, 2, 1, 16 * 64 + 64), 64),
+    (torch.zeros(2, 2, 1, 16 * 64, dtype=torch.uint8), 64),
+    (torch.zeros(2, 1, 1, 16 * 64 + 64, dtype=torch.uint8), 64),
+    (torch.zeros(2, 2, 1, 16 * 96 + 64, dtype=torch.uint8), 96),
+    (torch.zeros(2, 2, 2, 16 * 64 + 64, dtype=torch.uint8)[:, :, :1], 64),
+    (torch.zeros(2 * 2 * (16 * 64 + 64) + 1, dtype=torch.uint8)[1:].view(2, 2, 1, 16 * 64 + 64), 64),
+])
+def test_quantized_cache_refuses_other_pages(pages, d):
+    with pytest.raises(ValueError):
+        ops.QuantizedCache(pages, d)
+
+
+def _tree_args(d=64, q_heads=4, kv_heads=2, rows=3):
+    return dict(q=torch.zeros(rows, q_heads, d, dtype=BF16), cache=torch.zeros(4, 2, kv_heads, 16, d, dtype=BF16),
+                table=torch.zeros(4, dtype=I32), segments=torch.zeros(1, 5, dtype=I32), kv_heads=kv_heads, max_keys=64,
+                max_len=rows)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(q=torch.zeros(3, 4, 64)), "q must be BF16"),
+    (dict(q=torch.zeros(3, 256, dtype=BF16)), "q must be BF16"),
+    (dict(q=torch.zeros(3, 64, 4, dtype=BF16).transpose(1, 2)), "heads packed"),
+    (dict(q=torch.zeros(3, 4 * 64 + 4, dtype=BF16)[:, :256].view(3, 4, 64)), "multiple of 8"),
+    (dict(q=torch.zeros(3 * 256 + 1, dtype=BF16)[1:].view(3, 4, 64)), "16-byte"),
+    (dict(q=torch.zeros(3, 4, 96, dtype=BF16), cache=torch.zeros(4, 2, 2, 16, 96, dtype=BF16)), "head_dim"),
+    (dict(q=torch.zeros(3, 5, 64, dtype=BF16)), "multiple of the key/value heads"),
+    (dict(cache=torch.zeros(4, 2, 2, 16, 64)), "cache must be"),
+    (dict(cache=torch.zeros(4, 2, 3, 16, 64, dtype=BF16)), "cache must be"),
+    (dict(cache=ops.QuantizedCache.empty(4, 3, 64, device="cpu")), "other heads"),
+    (dict(segments=torch.zeros(1, 4, dtype=I32)), "segments"),
+    (dict(segments=torch.zeros(1, 5, dtype=torch.int64)), "segments"),
+    (dict(table=torch.zeros(4, dtype=torch.int64)), "table"),
+    (dict(max_keys=0), "max_keys"),
+    (dict(max_len=0), "max_len"),
+    (dict(keys_per_split=24), "multiple of 16"),
+    (dict(keys_per_split=0), "multiple of 16"),
+    (dict(mask=torch.zeros(2, 1, dtype=I32)), "mask"),
+    (dict(mask=torch.zeros(3, 0, dtype=I32)), "mask"),
+    (dict(mask=torch.zeros(3, dtype=I32)), "mask"),
+    (dict(out=torch.zeros(3, 4, 128, dtype=BF16)), "out must have"),
+    (dict(), "CUDA"),
+])
+def test_paged_tree_refusals(change, match):
+    with pytest.raises(ValueError, match=match):
+        ops.paged_tree(**{**_tree_args(), **change})
+
+
+def test_paged_decode_and_prefill_over_a_quantized_cache_refuse_bf16_options():
+    cache = ops.QuantizedCache.empty(4, 2, 64, device="cpu")
+    q, table, segs = torch.zeros(1, 4, 64, dtype=BF16), torch.zeros(4, dtype=I32), torch.zeros(1, 5, dtype=I32)
+    for option in (dict(warps=2), dict(stages=2), dict(counters=torch.zeros(2, dtype=I32))):
+        with pytest.raises(ValueError, match="BF16 pages"):
+            ops.paged_decode(q, cache, table, segs, 2, 16, **option)
+    with pytest.raises(ValueError, match="paged_tree"):
+        ops.paged_prefill(q, cache, table, segs, 2, torch.zeros(1, 2, dtype=I32))
+
+
+def _store_args(d=64, rows=3):
+    return dict(qkv=torch.zeros(rows, 8 * d, dtype=BF16), q_heads=4, kv_heads=2, head_dim=d, q_norm=None, k_norm=None,
+                eps=1e-6, positions=torch.zeros(rows, dtype=I32), inv_freq=torch.zeros(d // 2), attention_factor=1.0,
+                cache=ops.QuantizedCache.empty(4, 2, d, device="cpu"), slots=torch.zeros(rows, dtype=I32))
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(qkv=torch.zeros(3, 512)), "qkv must be BF16"),
+    (dict(qkv=torch.zeros(3, 511, dtype=BF16)), "qkv must be BF16"),
+    (dict(qkv=torch.zeros(512, 3, dtype=BF16).T), "unit column stride"),
+    (dict(qkv=torch.zeros(3, 516, dtype=BF16)[:, :512]), "aligned rows"),
+    (dict(q_norm=torch.zeros(64, dtype=BF16)), "come together"),
+    (dict(q_norm=torch.zeros(64), k_norm=torch.zeros(64)), "norm weights"),
+    (dict(positions=torch.zeros(3, dtype=torch.int64)), "positions"),
+    (dict(slots=torch.zeros(2, dtype=I32)), "slots"),
+    (dict(inv_freq=torch.zeros(16)), "inv_freq"),
+    (dict(rotary_dim=24), "rotary_dim"),
+    (dict(rotary_dim=0), "rotary_dim"),
+    (dict(rotary_dim=80), "rotary_dim"),
+    (dict(cache=ops.QuantizedCache.empty(4, 3, 64, device="cpu")), "other heads"),
+    (dict(cache=torch.zeros(4, 2, 2, 16, 64), interleaved=True), "cache must be"),
+    (dict(head_dim=96), "qkv must be BF16"),
+    (dict(), "CUDA"),
+])
+def test_store_refusals(change, match):
+    with pytest.raises(ValueError, match=match):
+        ops.qk_norm_rope_cache(**{**_store_args(), **change})
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(logits=torch.zeros(2, 10, dtype=torch.float16)), "FP32 or BF16"),
+    (dict(logits=torch.zeros(10)), "FP32 or BF16"),
+    (dict(logits=torch.zeros(2, 0)), "columns"),
+    (dict(logits=torch.zeros(10, 2).T), "unit column stride"),
+    (dict(logits=torch.zeros(1, 10).expand(2, 10)), "unit column stride"),
+    (dict(prompt=(torch.zeros(3, dtype=torch.int64), torch.zeros(3, dtype=I32))), "prompt tokens"),
+    (dict(output=(torch.zeros(3, dtype=I32), torch.zeros(2, dtype=I32))), "output starts"),
+    (dict(bias=(torch.zeros(3, dtype=I32), torch.zeros(3, dtype=I32))), "bias must be"),
+    (dict(bias=(torch.zeros(3, dtype=I32), torch.zeros(2), torch.zeros(3, dtype=I32))), "bias must be"),
+    (dict(repetition=torch.zeros(3)), "repetition"),
+    (dict(frequency=torch.zeros(2, dtype=BF16)), "frequency"),
+    (dict(presence=torch.zeros(2, 1)), "presence"),
+    (dict(allowed=torch.zeros(2, 0, dtype=I32)), "allowed"),
+    (dict(allowed=torch.zeros(1, 1, dtype=I32)), "allowed"),
+    (dict(out=torch.zeros(2, 10, dtype=BF16)), "out must have"),
+    (dict(out=torch.zeros(1, 10).expand(2, 10)), "out must have"),
+    (dict(), "CUDA"),
+])
+def test_process_logits_refusals(change, match):
+    with pytest.raises(ValueError, match=match):
+        ops.process_logits(**{**dict(logits=torch.zeros(2, 10)), **change})

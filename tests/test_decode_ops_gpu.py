@@ -1,0 +1,770 @@
+"""The decode-step operators against plain 64-bit forms: the quantizing store, attention of decode
+rows, chunks and drafted trees over BF16 and quantized pages, constrained logits, and one
+speculative step of all of them."""
+
+import random
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32, I32, F64 = torch.bfloat16, torch.float32, torch.int32, torch.float64
+E4M3 = torch.float8_e4m3fn
+DEV = "cuda"
+
+
+def _ops():
+    from furiosa_opt_models_b200 import ops
+
+    return ops
+
+
+def _half(dtype):
+    """Largest relative error of one rounding."""
+    return torch.finfo(dtype).eps / 2
+
+
+def _check():
+    torch.cuda.synchronize()
+    _ops().scratch(torch.device("cuda", 0)).check()
+
+
+def _status():
+    s = _ops().scratch(torch.device("cuda", 0)).status
+    torch.cuda.synchronize()
+    code = int(s[0].item())
+    s.zero_()
+    return code
+
+
+# ------------------------------------------------------------------------------- quantizing store
+
+
+def _front64(qkv, hq, hk, d, qn, kn, eps, pos, inv_freq, factor, rot, interleaved):
+    x = qkv.double().view(-1, hq + 2 * hk, d).cpu()
+    q, k, v = x[:, :hq], x[:, hq:hq + hk], x[:, hq + hk:]
+    out = []
+    for h, w in ((q, qn), (k, kn)):
+        if w is not None:
+            h = h / (h.square().mean(-1, keepdim=True) + eps).sqrt() * w.double().cpu()
+        h = h.clone()
+        a = (pos.double().cpu()[:, None] * inv_freq.double().cpu())[:, None]
+        i = torch.arange(rot // 2) * 2 if interleaved else torch.arange(rot // 2)
+        j = i + 1 if interleaved else i + rot // 2
+        xi, xj = h[..., i].clone(), h[..., j].clone()
+        h[..., i] = (xi * a.cos() - xj * a.sin()) * factor
+        h[..., j] = (xj * a.cos() + xi * a.sin()) * factor
+        out.append(h)
+    return out[0], out[1], v
+
+
+@pytest.mark.parametrize("rows,hq,hk,d,rot,interleaved,norm,quantized", [
+    (1, 16, 8, 128, 128, False, True, True),
+    (7, 4, 2, 64, 64, False, True, True),
+    (33, 14, 2, 64, 32, False, False, True),
+    (5, 6, 3, 128, 96, False, True, True),   # a rotation partner 6 lanes away
+    (9, 8, 1, 128, 16, True, True, True),
+    (200, 5, 5, 64, 64, True, False, True),
+    (3, 0, 2, 128, 128, False, False, True),  # keys and values alone
+    (700, 32, 8, 128, 128, True, True, True),
+    (6, 4, 2, 64, 32, True, True, False),
+    (6, 12, 4, 128, 64, False, False, False),
+])
+def test_store(rows, hq, hk, d, rot, interleaved, norm, quantized):
+    ops = _ops()
+    torch.manual_seed(rows)
+    wide = torch.randn(rows, (hq + 2 * hk) * d + 8, device=DEV).mul_(3).to(BF16)
+    qkv = wide[:, 8:] if rows % 2 else wide[:, :-8]  # rows of a wider tensor
+    qkv[0, -d:] = 0  # a value row of zeros
+    qn, kn = ((1 + 0.2 * torch.randn(d, device=DEV)).to(BF16) for _ in range(2)) if norm else (None, None)
+    pos = torch.randint(0, 131072, (rows,), device=DEV, dtype=I32)
+    inv_freq = 5e5 ** (-torch.arange(0, rot, 2, device=DEV, dtype=F32) / rot)
+    blocks = rows // 16 + 3
+    slots = torch.randperm(blocks * 16, device=DEV)[:rows].to(I32)
+    if rows > 4:
+        slots[2] = -1
+    if quantized:
+        cache = ops.QuantizedCache(torch.randint(0, 255, (blocks, 2, hk, 16 * d + 64), device=DEV).to(torch.uint8), d)
+        before = cache.pages.clone()
+    else:
+        cache = torch.randn(blocks, 2, hk, 16, d, device=DEV).to(BF16)
+        before = cache.clone()
+    q = ops.qk_norm_rope_cache(qkv, hq, hk, d, qn, kn, 1e-5, pos, inv_freq, 0.9, cache, slots, rotary_dim=rot,
+                               interleaved=interleaved)
+    _check()
+    rq, rk, rv = _front64(qkv, hq, hk, d, qn, kn, 1e-5, pos, inv_freq, 0.9, rot, interleaved)
+    # FP32 steps before the rounding: the norm's sum of d squares, its inverse root (2 ulp) and two
+    # products, an angle reduced to within pi (2^-24 * pi), sine and cosine (2 ulp), two products and
+    # a sum: under (d + 32) * 2^-24 of the pair's larger element, itself under the row's largest.
+    def slack(y):
+        return (d + 32) * 2.0 ** -24 * 2 * y.abs().amax(-1, keepdim=True)
+
+    assert ((q.double().cpu() - rq).abs() <= _half(BF16) * rq.abs() + slack(rq)).all()
+    touched = torch.zeros(blocks, 16, dtype=torch.bool)
+    for r, s in enumerate(slots.tolist()):
+        if s < 0:
+            continue
+        b, o = divmod(s, 16)
+        touched[b, o] = True
+        for which, y in ((0, rk[r]), (1, rv[r])):
+            if quantized:
+                scale = cache.scales[b, which, :, o].double().cpu()
+                want = y.abs().amax(-1).clamp_min(1e-10) / 448
+                assert ((scale - want).abs() <= want * (2 * (d + 32) * 2.0 ** -24 + 2.0 ** -22)).all()
+                got = cache.dequantize()[b, which, :, o].double().cpu()
+                # Half a step of the code: relative, or of the subnormal spacing 2^-9.
+                step = torch.maximum(_half(E4M3) * y.abs(), 2.0 ** -10 * scale[:, None])
+                assert ((got - y).abs() <= step * (1 + 2.0 ** -3) + slack(y)).all()
+            else:
+                got = cache[b, which, :, o].double().cpu()
+                assert ((got - y).abs() <= _half(BF16) * y.abs() + slack(y)).all()
+    # Every other slot is as it was.
+    if quantized:
+        old = ops.QuantizedCache(before, d)
+        same = (cache.codes == old.codes).all(-1) & (cache.pages[..., 16 * d:].unflatten(-1, (16, 4))
+                                                     == before[..., 16 * d:].unflatten(-1, (16, 4))).all(-1)
+    else:
+        same = (cache == before).all(-1)
+    assert (same.permute(0, 3, 1, 2).cpu() | touched[:, :, None, None]).all()
+
+
+def test_store_values_that_are_not_finite_and_bad_slots():
+    ops = _ops()
+    torch.manual_seed(1)
+    qkv = torch.randn(3, 4 * 64, device=DEV).to(BF16)
+    qkv[0, 2 * 64 + 3] = float("nan")  # the key head
+    qkv[1, 3 * 64 + 5] = float("inf")  # the value head
+    qkv[1, 3 * 64 + 6] = -float("inf")
+    cache = ops.QuantizedCache.empty(2, 1, 64)
+    slots = torch.tensor([3, 17, 32], device=DEV, dtype=I32)  # the last one lies past the cache
+    zero = torch.zeros(3, device=DEV, dtype=I32)
+    freq = torch.ones(8, device=DEV)
+    ops.qk_norm_rope_cache(qkv, 2, 1, 64, None, None, 1e-6, zero, freq, 1.0, cache, slots, rotary_dim=16)
+    assert _status() == 8
+    v = cache.dequantize()
+    # The rotation makes NaN of both elements of the NaN's pair, (3, 3 + 16 / 2).
+    assert v[0, 0, 0, 3].isnan().nonzero().flatten().tolist() == [3, 11]
+    assert v[1, 1, 0, 1].isnan().sum() == 2 and v[1, 1, 0, 1, 5:7].isnan().all()
+    # The others keep a scale of the finite ones.
+    y = qkv[1, 3 * 64:].double()
+    y = torch.where(y.isfinite(), y, 0)
+    keep = torch.arange(64, device=DEV)
+    keep = (keep != 5) & (keep != 6)
+    assert ((v[1, 1, 0, 1].double() - y).abs() <= 2.0 ** -4 * y.abs() + y.abs().max() * 2.0 ** -18)[keep].all()
+    assert torch.count_nonzero(v.nan_to_num(1.0)[:, :, 0].amax(-1)) == 4  # two rows' keys and values, nothing else
+
+
+# ------------------------------------------------------------------------------------- attention
+
+
+def _paged(lens, cached, hk, d, quantized, gen, spare=3):
+    """(cache, table, segments, values in 64 bits) with scattered blocks; the slots past each
+    sequence's end and the spare blocks hold NaN."""
+    ops = _ops()
+    segs, row, start = [], 0, 0
+    for n, c in zip(lens, cached):
+        nb = (n + c + 15) // 16
+        segs.append((row, n, c, start, nb))
+        row, start = row + n, start + nb
+    blocks = start + spare
+    x = torch.randn(blocks, 2, hk, 16, d, generator=gen) * 0.7
+    x[:, 1] *= torch.rand(blocks, hk, 16, 1, generator=gen) * 3 + 0.01  # values of unequal sizes
+    table = torch.randperm(blocks, generator=gen)[:start]
+    if quantized:
+        pages = torch.zeros(blocks, 2, hk, 16 * d + 64, dtype=torch.uint8)
+        scale = x.abs().amax(-1).clamp_min(1e-10) / 448
+        codes = (x / scale[..., None]).clamp(-448, 448).to(E4M3)
+        pages[..., :16 * d] = codes.view(torch.uint8).flatten(3)
+        pages[..., 16 * d:] = scale.view(torch.uint8)
+        values = codes.double() * scale.double()[..., None]
+    else:
+        pages = x.to(BF16)
+        values = pages.double()
+    used = torch.zeros(blocks, 16, dtype=torch.bool)
+    for _, n, c, s, nb in segs:
+        for b in range(nb):
+            used[table[s + b], :max(0, min(16, n + c - 16 * b))] = True
+    for b, o in (~used).nonzero().tolist():
+        if quantized:
+            pages[b, :, :, o * d:(o + 1) * d] = 0x7F
+            pages[b, :, :, 16 * d + 4 * o:16 * d + 4 * o + 4] = torch.tensor(
+                [float("nan")]).view(torch.uint8)
+        else:
+            pages[b, :, :, o] = float("nan")
+    cache = ops.QuantizedCache(pages.to(DEV), d) if quantized else pages.to(DEV)
+    return (cache, table.to(I32).to(DEV), torch.tensor(segs, dtype=I32).reshape(-1, 5).to(DEV), values, table, segs)
+
+
+def _attend64(q, values, table, segs, scale, mask=None, causal=True):
+    """(outputs, tolerances) of the formula in 64 bits. ``mask``: per segment, bool [len, len]."""
+    rows, hq, d = q.shape
+    hk = values.shape[2]
+    out, weight, err = (torch.zeros(rows, hq, d, dtype=F64) for _ in range(3))
+    for i, (row, n, c, start, nb) in enumerate(segs):
+        if n == 0:
+            continue
+        pages = values[table[start:start + nb]]
+        k, v = (pages[:, w].permute(0, 2, 1, 3).reshape(-1, hk, d)[:n + c] for w in (0, 1))
+        see = torch.ones(n, n + c, dtype=torch.bool)
+        see[:, c:] = torch.tril(torch.ones(n, n)).bool() if mask is None else mask[i]
+        for h in range(hq):
+            kh, vh = k[:, h * hk // hq], v[:, h * hk // hq]
+            qh = q[row:row + n, h].double()
+            s = (qh @ kh.T * scale).masked_fill(~see, -torch.inf)
+            p = torch.softmax(s, -1).nan_to_num(0.0) * see
+            seen = torch.where(see.any(0)[:, None], vh, 0.0)
+            p_v = torch.where(p[..., None] > 0, p[..., None] * seen, 0.0)
+            out[row:row + n, h] = p_v.sum(1)
+            weight[row:row + n, h] = p_v.abs().sum(1)
+            err[row:row + n, h] = ((qh.abs() @ kh.abs().nan_to_num(0.0).T) * scale).masked_fill(~see, 0).amax(-1, keepdim=True)
+    return out, weight, err
+
+
+def _tolerance(ref, weight, err, d, quantized):
+    """One rounding of the output, one of each weight (FP16 over codes, BF16 over BF16), and the
+    scores' FP32 sums of d products (and two scalings), each off by 2^-24 of the sum of magnitudes;
+    a weight and its sum feel that twice. ex2 and lg2 add 2^-21 each."""
+    return _half(BF16) * ref.abs() + weight * (
+        _half(torch.float16 if quantized else BF16) + 2 * (d + 4) * 2.0 ** -24 * err + 2.0 ** -20)
+
+
+def _random_masks(lens, gen, empty=False):
+    """Per segment bool [len, len]; random bits (not a tree), some rows empty."""
+    ms = []
+    for n in lens:
+        m = torch.rand(n, n, generator=gen) < 0.5
+        if empty and n:
+            m[0] = False
+        ms.append(m)
+    return ms
+
+
+def _pack(ms, extra=0):
+    words = max([1] + [(m.shape[0] + 31) // 32 for m in ms]) + extra
+    rows = []
+    for m in ms:
+        for r in m.tolist():
+            b = sum(1 << j for j, x in enumerate(r) if x)
+            rows.append([(b >> 32 * w) & 0xFFFFFFFF for w in range(words)])
+    return torch.tensor(rows, dtype=torch.int64).to(I32).to(DEV)
+
+
+HEADS = [(16, 8, 128), (32, 8, 128), (8, 8, 64), (14, 2, 64), (12, 1, 128), (64, 2, 64)]
+
+
+@pytest.mark.parametrize("split", [None, 16, 64, 4096])
+@pytest.mark.parametrize("hq,hk,d", HEADS)
+def test_decode_over_quantized_pages(hq, hk, d, split):
+    ops = _ops()
+    gen = torch.Generator().manual_seed(hq * d)
+    cached = [0, 1, 14, 15, 16, 100, 511, 1000, 2047]
+    cache, table, segs, values, tab, sl = _paged([1] * len(cached), cached, hk, d, True, gen)
+    q = (torch.randn(len(cached), hq, d, generator=gen) * 1.5).to(BF16)
+    out = ops.paged_decode(q.to(DEV), cache, table, segs, hk, 2048, keys_per_split=split)
+    _check()
+    ref, weight, err = _attend64(q, values, tab, sl, d ** -0.5)
+    assert ((out.double().cpu() - ref).abs() <= _tolerance(ref, weight, err, d, True)).all()
+
+
+LENS = [([1, 2, 5, 16, 33, 64, 7], [0, 1, 15, 16, 100, 700, 257]), ([40, 130, 1], [0, 300, 31]), ([300], [5]), ([3], [0])]
+
+
+@pytest.mark.parametrize("quantized", [True, False], ids=["e4m3", "bf16"])
+@pytest.mark.parametrize("split", [None, 32, 2048])
+@pytest.mark.parametrize("hq,hk,d", HEADS)
+def test_tree_masks(hq, hk, d, split, quantized):
+    ops = _ops()
+    for case, (lens, cached) in enumerate(LENS):
+        gen = torch.Generator().manual_seed(hq + d + case)
+        cache, table, segs, values, tab, sl = _paged(lens, cached, hk, d, quantized, gen)
+        q = (torch.randn(sum(lens), hq, d, generator=gen) * 1.5).to(BF16)
+        ms = _random_masks(lens, gen, empty=True)
+        bound = max(n + c for n, c in zip(lens, cached))
+        out = ops.paged_tree(q.to(DEV), cache, table, segs, hk, bound + 9 * case, max(lens) + case, mask=_pack(ms, case),
+                             keys_per_split=split)
+        _check()
+        ref, weight, err = _attend64(q, values, tab, sl, d ** -0.5, mask=ms)
+        assert ((out.double().cpu() - ref).abs() <= _tolerance(ref, weight, err, d, quantized)).all()
+        if cached[0] == 0 and case != 2:
+            assert torch.count_nonzero(out[0]) == 0  # a first token that sees nothing
+
+
+@pytest.mark.parametrize("quantized", [True, False], ids=["e4m3", "bf16"])
+@pytest.mark.parametrize("hq,hk,d", HEADS)
+def test_chunks_are_causal_without_a_mask(hq, hk, d, quantized):
+    ops = _ops()
+    gen = torch.Generator().manual_seed(5)
+    lens, cached = [17, 1, 129, 40], [0, 64, 250, 1]
+    cache, table, segs, values, tab, sl = _paged(lens, cached, hk, d, quantized, gen)
+    wide = (torch.randn(sum(lens), hq + 1, d, generator=gen)).to(BF16)
+    q = wide[:, :hq]  # rows of a wider tensor
+    held = torch.full((sum(lens), hq + 2, d), 7.0, dtype=BF16, device=DEV)
+    got = ops.paged_tree(q.to(DEV) if hq % 2 else wide.to(DEV)[:, :hq], cache, table, segs, hk, 400, 129, scale=0.2,
+                         out=held[:, :hq])
+    _check()
+    assert got.data_ptr() == held.data_ptr() and (held[:, hq:] == 7).all()
+    ref, weight, err = _attend64(q, values, tab, sl, 0.2)
+    assert ((got.double().cpu() - ref).abs() <= _tolerance(ref, weight, err, d, quantized)).all()
+
+
+@pytest.mark.parametrize("quantized", [True, False], ids=["e4m3", "bf16"])
+@pytest.mark.parametrize("n", [6, 70])
+def test_what_a_row_does_not_see_does_not_reach_it(n, quantized):
+    """NaN and infinities in drafted nodes stay with the rows that see them."""
+    ops = _ops()
+    gen = torch.Generator().manual_seed(3)
+    hq, hk, d = 8, 2, 128
+    lens, cached = [n], [37]
+    cache, table, segs, values, tab, sl = _paged(lens, cached, hk, d, quantized, gen)
+    key, value = cached[0] + 2, cached[0] + 4  # nodes 2 (a NaN key) and 4 (values)
+    pages = cache.pages if quantized else cache
+
+    def at(pos):
+        return tab[pos // 16], pos % 16
+
+    b, o = at(key)
+    values[b, 0, :, o, 9] = float("nan")
+    if quantized:
+        pages[b, 0, :, o * d + 9] = 0x7F
+    else:
+        pages[b, 0, :, o, 9] = float("nan")
+    b, o = at(value)
+    values[b, 1, :, o, 11] = float("nan")
+    if quantized:
+        pages[b, 1, :, o * d + 11] = 0xFF
+    else:
+        pages[b, 1, :, o, 11] = float("nan")
+        pages[b, 1, :, o, 12] = float("inf")
+        values[b, 1, :, o, 12] = float("inf")
+    ms = [torch.eye(n, dtype=torch.bool)]
+    ms[0][1, 2] = ms[0][3, 4] = ms[0][n - 1, 0] = True  # row 1 sees the key, row 3 the values
+    q = torch.randn(n, hq, d, generator=gen).to(BF16)
+    for split in (None, 16):
+        out = ops.paged_tree(q.to(DEV), cache, table, segs, hk, n + 37, n, mask=_pack(ms), keys_per_split=split).cpu()
+        _check()
+        clean = [r for r in range(n) if r not in (1, 2, 3, 4)]
+        ref, weight, err = _attend64(q, values, tab, sl, d ** -0.5, mask=ms)
+        tol = _tolerance(ref, weight, err, d, quantized)
+        assert ((out.double() - ref).abs() <= tol)[clean].all()
+        assert out[[1, 2]].isnan().all()
+        for r in (3, 4):
+            assert out[r, :, 11].isnan().all()
+            fine = [c for c in range(d) if c != 11 and (quantized or c != 12)]
+            assert ((out[r].double() - ref[r]).abs() <= tol[r])[:, fine].all()
+            if not quantized:
+                assert (out[r, :, 12] == float("inf")).all()
+
+
+@pytest.mark.parametrize("quantized", [True, False], ids=["e4m3", "bf16"])
+def test_scores_of_a_wide_range(quantized):
+    """Scores that rise by hundreds along the keys, and rows of large and of tiny queries."""
+    ops = _ops()
+    gen = torch.Generator().manual_seed(11)
+    hq, hk, d = 8, 2, 128
+    for n, split in ((1, 256), (1, 4096), (40, 4096), (40, 512)):
+        cache, table, segs, values, tab, sl = _paged([n], [1500], hk, d, quantized, gen)
+        q = torch.randn(n, hq, d, generator=gen) * torch.logspace(-30, 2.5, hq)[:, None]
+        q = q.to(BF16)
+        out = ops.paged_tree(q.to(DEV), cache, table, segs, hk, 1540, n, keys_per_split=split)
+        _check()
+        ref, weight, err = _attend64(q, values, tab, sl, d ** -0.5)
+        assert ((out.double().cpu() - ref).abs() <= _tolerance(ref, weight, err, d, quantized)).all()
+
+
+@pytest.mark.parametrize("quantized", [True, False], ids=["e4m3", "bf16"])
+@pytest.mark.parametrize("n", [2, 48])
+def test_segments_that_do_not_fit_the_call(n, quantized):
+    """Fields past the call's bounds give zeros and a status; rows of no segment stay as they were."""
+    ops = _ops()
+    gen = torch.Generator().manual_seed(2)
+    hq, hk, d = 16, 8, 64
+    cache, table, segs, values, tab, sl = _paged([n, n, n], [20, 30, 200], hk, d, quantized, gen)
+    q = torch.randn(3 * n + 2, hq, d, generator=gen).to(BF16).to(DEV)
+    whole = ops.paged_tree(q, cache, table, segs, hk, 200 + n, n)
+    _check()
+
+    def call(change=None, max_keys=200 + n, max_len=n):
+        s = segs.clone()
+        if change:
+            s[1, change[0]] = change[1]
+        out = torch.full_like(q, 3.0)
+        ops.paged_tree(q, cache, table, s, hk, max_keys, max_len, out=out)
+        return out, _status()
+
+    for change in ((2, -1), (2, 500), (3, -4), (3, 100000), (4, 1), (4, 1 << 30), (1, n + 1), (2, (1 << 31) - 1)):
+        out, code = call(change)
+        assert code == 7, change
+        rows = slice(n, 2 * n + (1 if change[0] == 1 else 0))
+        other = 2 * n + (1 if change[0] == 1 else 0)
+        if change[0] != 1:  # (a longer segment also covers the next one's first row)
+            assert torch.count_nonzero(out[rows]) == 0, change
+        assert torch.equal(out[:n], whole[:n]) and torch.equal(out[other:3 * n], whole[other:3 * n])
+        assert (out[3 * n:] == 3).all()
+    for change in ((0, -1), (0, 3 * n + 2), (1, -3), (0, (1 << 31) - 1)):  # rows outside q: nothing is written for them
+        out, code = call(change)
+        assert code == 7, change
+        assert (out[n:2 * n] == 3).all() and torch.equal(out[:n], whole[:n])
+    out, code = call((1, 0))  # an empty segment is nothing
+    assert code == 0 and (out[n:2 * n] == 3).all()
+    out, code = call(max_keys=100 + n)
+    assert code == 7 and torch.count_nonzero(out[2 * n:3 * n]) == 0
+    # A block ID outside the cache reads as zeros.
+    bad = table.clone()
+    bad[sl[2][3]] = 1 << 20
+    bad[sl[2][3] + 1] = -7
+    out = ops.paged_tree(q, cache, bad, segs, hk, 200 + n, n)
+    assert _status() == 8
+    assert torch.isfinite(out[:3 * n].float()).all()
+    assert torch.equal(out[:2 * n], whole[:2 * n])
+
+
+def test_a_fixed_split_gives_the_same_bits_in_any_batch():
+    ops = _ops()
+    gen = torch.Generator().manual_seed(8)
+    hq, hk, d = 32, 8, 128
+    cache, table, segs, _, _, sl = _paged([1] * 5 + [20], [900, 40, 3, 1777, 512, 600], hk, d, True, gen)
+    q = torch.randn(25, hq, d, generator=gen).to(BF16).to(DEV)
+    whole = ops.paged_tree(q, cache, table, segs, hk, 1778, 20, keys_per_split=512)
+    again = ops.paged_tree(q, cache, table, segs, hk, 1778, 20, keys_per_split=512)
+    assert torch.equal(whole, again)
+    one = ops.paged_tree(q, cache, table, segs[3:4].contiguous(), hk, 1778, 20, keys_per_split=512)
+    _check()
+    assert torch.equal(whole[3], one[3])
+
+
+def test_offsets_past_32_bits():
+    """Pages beyond 2^32 bytes of the cache: a quantized cache of 4.6 GB whose last blocks are used."""
+    ops = _ops()
+    hq, hk, d = 16, 8, 128
+    blocks = (1 << 32) // (2 * hk * (16 * d + 64)) + 9000
+    pages = torch.zeros(blocks, 2, hk, 16 * d + 64, dtype=torch.uint8, device=DEV)
+    cache = ops.QuantizedCache(pages, d)
+    gen = torch.Generator().manual_seed(4)
+    small, table, segs, values, tab, sl = _paged([1, 40], [70, 90], hk, d, True, gen)
+    far = blocks - small.pages.shape[0]
+    pages[far:] = small.pages
+    q = torch.randn(41, hq, d, generator=gen).to(BF16)
+    out = ops.paged_tree(q.to(DEV), cache, table + far, segs, hk, 130, 40)
+    _check()
+    ref, weight, err = _attend64(q, values, tab, sl, d ** -0.5)
+    assert ((out.double().cpu() - ref).abs() <= _tolerance(ref, weight, err, d, True)).all()
+    # The store reaches them too.
+    qkv = torch.randn(2, (hq + 2 * hk) * d, device=DEV).to(BF16)
+    slots = torch.tensor([blocks * 16 - 1, 5], device=DEV, dtype=I32)
+    pos = torch.zeros(2, device=DEV, dtype=I32)
+    ops.qk_norm_rope_cache(qkv, hq, hk, d, None, None, 1e-6, pos, torch.ones(64, device=DEV), 1.0, cache, slots)
+    _check()
+    y = qkv[0].view(-1, d)[-hk:].float()
+    got = cache.codes[-1, 1, :, 15].view(E4M3).float() * cache.scales[-1, 1, :, 15, None]
+    assert ((got - y).abs() <= 2.0 ** -4 * y.abs() + 2.0 ** -18 * y.abs().amax(-1, keepdim=True)).all()
+
+
+# ---------------------------------------------------------------------------------------- logits
+
+
+def _logits64(x, prompt, output, rep, freq, pres, bias, allowed):
+    """Per row python lists; x [rows, vocab] FP64. Returns (values, magnitudes for the tolerance)."""
+    x = x.clone()
+    size = x.abs()
+    rows, vocab = x.shape
+    for r in range(rows):
+        inside = [t for t in output[r] if 0 <= t < vocab]
+        listed = set(inside) | {t for t in prompt[r] if 0 <= t < vocab} if rep is not None else set()
+        for t in listed:
+            x[r, t] = x[r, t] / rep[r] if x[r, t] > 0 else x[r, t] * rep[r]
+            size[r, t] += x[r, t].abs()
+        for t in set(inside):
+            n = inside.count(t)
+            f = freq[r] * n if freq is not None else 0.0
+            g = pres[r] if pres is not None else 0.0
+            x[r, t] -= f + g
+            size[r, t] += abs(f) + abs(g)
+        for t, v in dict(bias[r]).items():
+            if 0 <= t < vocab:
+                x[r, t] += v
+                size[r, t] += abs(v)
+        if allowed is not None:
+            x[r, ~allowed[r]] = -torch.inf
+    return x, size
+
+
+def _csr(lists, kind=I32, pick=lambda v: v):
+    flat = [pick(v) for row in lists for v in row]
+    starts = [0]
+    for row in lists:
+        starts.append(starts[-1] + len(row))
+    return torch.tensor(flat, dtype=kind, device=DEV), torch.tensor(starts, dtype=I32, device=DEV)
+
+
+def _bits(allowed):
+    rows, vocab = allowed.shape
+    words = (vocab + 31) // 32
+    full = torch.zeros(rows, words * 32, dtype=torch.int64)
+    full[:, :vocab] = allowed.long()
+    return (full.view(rows, words, 32) << torch.arange(32)).sum(-1).to(I32).to(DEV)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab,features", [
+    (1, 1, "pb"), (3, 7, "pbm"), (2, 31, "m"), (5, 1000, "pbm"), (2, 1001, "p"), (3, 32000, "b"), (2, 151936, "pbm"),
+    (2, 262145, "pbm"), (4, 50257, ""), (1, 700001, "pbm"), (2, 33, "f"), (2, 4099, "r"),
+])
+def test_process_logits(rows, vocab, features, dtype):
+    ops = _ops()
+    rng = random.Random(rows * vocab)
+    gen = torch.Generator().manual_seed(vocab)
+    pad = rng.randrange(0, 9)
+    wide = torch.randn(rows, vocab + pad, generator=gen).mul(4).to(dtype).to(DEV)
+    x = wide[:, pad:]  # rows that begin at any place
+    if rows > 1 and vocab > 3:
+        x[1, 2] = float("nan")
+    few = [rng.randrange(vocab) for _ in range(20)]
+    lists = lambda n: [[rng.choice(few) if rng.random() < 0.5 else rng.randrange(vocab) for _ in range(rng.randrange(n))]  # noqa: E731
+                       + [vocab, -1, vocab + 5] for _ in range(rows)]
+    prompt, output = lists(300), lists(2000)
+    output[-1] = []
+    rep = freq = pres = None
+    if "p" in features or "r" in features:
+        rep = torch.rand(rows, generator=gen) + 0.8
+    if "p" in features or "f" in features:
+        freq = torch.rand(rows, generator=gen) - 0.2
+    if "p" in features:
+        pres = torch.rand(rows, generator=gen)
+    bias = [[(rng.randrange(-1, vocab + 1), rng.uniform(-9, 9)) for _ in range(rng.randrange(40))] for _ in range(rows)]
+    if "b" not in features:
+        bias = [[] for _ in range(rows)]
+    elif vocab > 3:
+        bias[0] += [(3, 1.0), (3, 2.0), (3, -0.5)]  # the last one counts
+    bias = [[(t, float(torch.tensor(v, dtype=F32))) for t, v in row] for row in bias]
+    allowed = None
+    if "m" in features:
+        allowed = torch.rand(rows, vocab, generator=gen) < torch.tensor([0.9, 0.01, 0.5, 0.0, 0.3])[:rows, None]
+        if rows > 2:
+            allowed[2] = False  # nothing is left
+            allowed[0] = False
+            allowed[0, vocab - 1] = True
+    out = torch.full((rows, vocab + 3), 9.0, dtype=dtype, device=DEV)[:, :vocab]
+    kw = dict(prompt=_csr(prompt), output=_csr(output), allowed=None if allowed is None else _bits(allowed))
+    for name, v in (("repetition", rep), ("frequency", freq), ("presence", pres)):
+        if v is not None:
+            kw[name] = v.to(DEV)
+    if "b" in features:
+        bt, bs = _csr(bias, pick=lambda v: v[0])
+        kw["bias"] = (bt, _csr(bias, kind=F32, pick=lambda v: v[1])[0], bs)
+    index, value = ops.process_logits(x, out=out, **kw)
+    greedy = ops.process_logits(x, **kw)
+    _check()
+    assert torch.equal(index, greedy[0]) and torch.equal(value, greedy[1])
+    d64 = lambda v: None if v is None else v.double()  # noqa: E731
+    ref, size = _logits64(x.double().cpu(), prompt, output, d64(rep), d64(freq), d64(pres), bias, allowed)
+    # Five FP32 steps (a product, a quotient or product, two differences, a sum), and one rounding
+    # of the stored logit.
+    got = out.double().cpu()
+    tol = 5 * 2.0 ** -24 * size + (_half(BF16) * ref.abs() if dtype == BF16 else 0)
+    inf = ref == -torch.inf
+    assert torch.equal(got == -torch.inf, inf) and torch.equal(got.isnan(), ref.isnan())
+    real = ~inf & ~ref.isnan()
+    assert ((got - ref).abs() <= tol)[real].all()
+    assert torch.all(out.as_strided((rows, 3), (vocab + 3, 1), out.storage_offset() + vocab) == 9)
+    for r in range(rows):
+        ok = real[r]
+        if not ok.any():
+            assert index[r] == -1 and value[r] == -torch.inf
+            continue
+        i = int(index[r])
+        assert ok[i] and (value[r].double().cpu() - ref[r, i]).abs() <= 5 * 2.0 ** -24 * size[r, i]
+        assert (ref[r, ok] <= ref[r, i] + (5 * 2.0 ** -24 * size[r])[ok] + 5 * 2.0 ** -24 * size[r, i]).all()
+        if dtype == F32:
+            best = out[r].cpu()[ok].max()
+            assert value[r].cpu() == best and i == int((out[r].cpu() == best).nonzero()[0])
+
+
+def test_process_logits_ties_in_place_and_bad_lists():
+    ops = _ops()
+    x = torch.zeros(2, 5000, device=DEV)
+    x[:, [17, 18, 4999]] = 3.0
+    index, value = ops.process_logits(x)
+    assert index.tolist() == [17, 17] and value.tolist() == [3.0, 3.0]
+    # In place: the same as into another tensor.
+    lists = (torch.tensor([17, 17, 40], device=DEV, dtype=I32), torch.tensor([0, 3, 3], device=DEV, dtype=I32))
+    freq = torch.full((2,), 0.5, device=DEV)
+    other = torch.empty_like(x)
+    a = ops.process_logits(x, output=lists, frequency=freq, out=other)
+    b = ops.process_logits(x, output=lists, frequency=freq, out=x)
+    _check()
+    assert torch.equal(x, other) and torch.equal(a[0], b[0]) and a[0].tolist() == [18, 17]
+    assert x[0, 17] == 2.0 and x[0, 40] == -0.5 and x[1, 40] == 0.0
+    # Starts that leave the list read as an empty list.
+    for starts in ([0, 3, 4], [2, 1, 3], [-1, 2, 3]):
+        bad = (lists[0], torch.tensor(starts, device=DEV, dtype=I32))
+        ops.process_logits(x, output=bad, frequency=freq, out=other)
+        assert _status() == 7
+        rows = [r for r in range(2) if not 0 <= starts[r] <= starts[r + 1] <= 3]
+        assert torch.equal(other[rows], x[rows])
+    none = ops.process_logits(x[:0], out=other[:0])
+    assert none[0].shape == (0,)
+
+
+# ------------------------------------------------------------------------------- a run of them all
+
+
+class _Step:
+    """One speculative step of a one-layer model over a quantized cache: drafted rows are projected
+    to q/k/v, stored, attended with their tree and scored under penalties and a grammar mask."""
+
+    def __init__(self, seed, vocab=2048, hq=8, hk=2, d=64, hidden=256):
+        g = torch.Generator().manual_seed(seed)
+        rand = lambda *s: torch.randn(*s, generator=g).mul(s[-1] ** -0.5).to(BF16).to(DEV)  # noqa: E731
+        self.hq, self.hk, self.d, self.vocab = hq, hk, d, vocab
+        self.emb = torch.randn(vocab, hidden, generator=g).to(BF16).to(DEV)
+        self.w_qkv, self.w_o, self.head = rand((hq + 2 * hk) * d, hidden), rand(hidden, hq * d), rand(vocab, hidden)
+        self.qn, self.kn = torch.ones(d, dtype=BF16, device=DEV), torch.ones(d, dtype=BF16, device=DEV)
+        self.inv_freq = 1e4 ** (-torch.arange(0, d, 2, device=DEV, dtype=F32) / d)
+        self.blocks = 24
+        self.cache = _ops().QuantizedCache.empty(self.blocks, hk, d)
+
+    def __call__(self, tokens, positions, slots, table, segments, max_keys, max_len, mask, **logit_args):
+        ops = _ops()
+        qkv = ops.gemm(ops.embedding(tokens, self.emb), self.w_qkv)
+        q = ops.qk_norm_rope_cache(qkv, self.hq, self.hk, self.d, self.qn, self.kn, 1e-6, positions, self.inv_freq, 1.0,
+                                   self.cache, slots)
+        o = ops.paged_tree(q, self.cache, table, segments, self.hk, max_keys, max_len, mask=mask)
+        logits = ops.gemm(ops.gemm(o.flatten(1), self.w_o), self.head, epilogue=ops.EPI_F32)
+        return (o, logits) + ops.process_logits(logits, **logit_args)
+
+
+def _step_inputs(step, seed):
+    """Two sequences of 50 and 33 positions, a tree of 7 and one of 4 drafted nodes."""
+    rng = random.Random(seed)
+    hist = [50, 33]
+    parents = [[-1, 0, 0, 1, 1, 2, 5], [-1, 0, 1, -1]]
+    blocks = rng.sample(range(step.blocks), 10)
+    tables = [blocks[:5], blocks[5:]]
+    i32 = lambda v: torch.tensor(v, dtype=I32, device=DEV)  # noqa: E731
+    slot = lambda s, p: tables[s][p // 16] * 16 + p % 16  # noqa: E731
+    prompt = dict(
+        tokens=i32([rng.randrange(step.vocab) for _ in range(sum(hist))]),
+        positions=i32([p for n in hist for p in range(n)]),
+        slots=i32([slot(s, p) for s, n in enumerate(hist) for p in range(n)]),
+        table=i32(blocks), segments=i32([[0, 50, 0, 0, 4], [50, 33, 0, 5, 3]]), max_keys=64, max_len=50, mask=None)
+    depth = []
+    for tree in parents:
+        d = []
+        for p in tree:
+            d.append(0 if p < 0 else d[p] + 1)
+        depth.append(d)
+    drafted = dict(
+        tokens=i32([rng.randrange(step.vocab) for _ in range(11)]),
+        positions=i32([hist[s] + x for s in range(2) for x in depth[s]]),
+        slots=i32([slot(s, hist[s] + j) for s, t in enumerate(parents) for j in range(len(t))]),
+        table=i32(blocks), segments=i32([[0, 7, 50, 0, 5], [7, 4, 33, 5, 5]]), max_keys=80, max_len=8,
+        mask=_ops().tree_mask(parents).to(DEV))
+    words = step.vocab // 32
+    drafted.update(
+        output=(i32([rng.randrange(step.vocab) for _ in range(11 * 6)]), i32([6 * r for r in range(12)])),
+        presence=torch.rand(11, device=DEV), frequency=torch.rand(11, device=DEV),
+        allowed=torch.randint(-2 ** 31, 2 ** 31, (11, words), device=DEV, dtype=torch.int64).to(I32))
+    return prompt, drafted, parents
+
+
+def test_a_speculative_step():
+    ops = _ops()
+    step = _Step(0)
+    prompt, drafted, parents = _step_inputs(step, 0)
+    step(**prompt)
+    o, logits, index, value = step(**drafted)
+    _check()
+    # The drafted rows' attention from what the cache holds.
+    qkv = ops.gemm(ops.embedding(drafted["tokens"], step.emb), step.w_qkv)
+    rq, _, _ = _front64(qkv, step.hq, step.hk, step.d, step.qn, step.kn, 1e-6, drafted["positions"], step.inv_freq, 1.0,
+                        step.d, False)
+    values = (step.cache.codes.view(E4M3).double() * step.cache.scales.double()[..., None]).cpu()
+    ms = [torch.zeros(len(t), len(t), dtype=torch.bool) for t in parents]
+    for m, tree in zip(ms, parents):
+        for i, p in enumerate(tree):
+            if p >= 0:
+                m[i] |= m[p]
+            m[i, i] = True
+    ref, weight, err = _attend64(rq.to(BF16), values, drafted["table"].cpu().long(), drafted["segments"].tolist(),
+                                 step.d ** -0.5, mask=ms)
+    # q rounds to BF16 in the kernel from FP32 and here from FP64: a step apart at most, which moves
+    # each score by 2^-8 of its sum of magnitudes at worst.
+    tol = _tolerance(ref, weight, err, step.d, True) + 2 * _half(BF16) * 2 * weight * err
+    assert ((o.double().cpu() - ref).abs() <= tol).all()
+    lists = drafted["output"][0].view(11, 6).tolist()
+    bits = (drafted["allowed"].cpu().long()[:, :, None] >> torch.arange(32)).flatten(1) & 1 == 1
+    want, size = _logits64(logits.double().cpu(), [[]] * 11, lists, None, drafted["frequency"].double().cpu(),
+                           drafted["presence"].double().cpu(), [[]] * 11, bits)
+    top = want.amax(-1)
+    assert ((value.double().cpu() - top).abs() <= 5 * 2.0 ** -24 * size.amax(-1)).all()
+    assert bits[torch.arange(11), index.cpu().long()].all()
+
+
+def test_a_captured_step_replays_on_other_inputs_and_streams():
+    """Two graphs of the step, replayed in turn and side by side on two streams, against eager calls."""
+    ops = _ops()
+    ops.scratch(torch.device("cuda", 0))
+    steps = [_Step(1), _Step(2)]
+    ins = [_step_inputs(s, i) for i, s in enumerate(steps)]
+    for s, (prompt, drafted, _) in zip(steps, ins):
+        s(**prompt)
+        s(**drafted)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for s, (_, drafted, _) in zip(steps, ins):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(s(**drafted))
+        graphs.append(g)
+    for seed in (5, 6):
+        wants = []
+        for s, (_, drafted, _) in zip(steps, ins):
+            gen = torch.Generator().manual_seed(seed)
+            drafted["tokens"].copy_(torch.randint(0, s.vocab, (11,), generator=gen).to(I32))
+            before = s.cache.pages.clone()
+            wants.append([t.clone() for t in s(**drafted)])
+            s.cache.pages.copy_(before)
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in graphs]
+        for _ in range(3):
+            for g, st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    g.replay()
+        torch.cuda.synchronize()
+        for want, got in zip(wants, outs):
+            assert all(torch.equal(a, b) for a, b in zip(want, got))
+    _check()
+
+
+def test_calls_run_on_the_current_stream():
+    ops = _ops()
+    gen = torch.Generator().manual_seed(9)
+    cache, table, segs, _, _, _ = _paged([1] * 4, [500, 600, 700, 2000], 8, 128, True, gen)
+    q = torch.randn(4, 16, 128, generator=gen).to(BF16).to(DEV)
+    want = ops.paged_decode(q, cache, table, segs, 8, 2001)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    big = torch.randn(4096, 4096, device=DEV)
+    late = torch.zeros_like(q)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            big = (big @ big).tanh()
+        late.copy_(q)  # arrives behind the products
+        got = ops.paged_decode(late, cache, table, segs, 8, 2001)
+    side.synchronize()
+    _check()
+    assert torch.equal(want, got)
+
+
+def test_a_first_call_is_not_captured(monkeypatch):
+    """The device's status word is laid out by the first call, outside of any graph."""
+    ops = _ops()
+    monkeypatch.setattr("furiosa_opt_models_b200.ops.decode._scratch", {})
+    x = torch.zeros(1, 8, device=DEV)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = x + 1  # noqa: F841
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            ops.process_logits(x)
