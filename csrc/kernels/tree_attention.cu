@@ -6,22 +6,25 @@
 // Row i of a segment sees the whole history and the appended rows j its mask names (or j <= i). A
 // row that sees nothing gets zeros. What a row does not see does not reach it, NaN included.
 //
-// This is the mma.sync form, one CTA per (segment, key/value head, 16 (token, head) rows, split of
-// the keys); its warps take the split's 16-key pages in turn, each streaming them through its own
-// cp.async ring, and merge at the end. Splits meet in a second kernel, in split order.
+// This is the mma.sync form, one CTA per (segment, key/value head, tile of 8 or 16 (token, head)
+// rows, split of the keys); its warps take the split's 16-key pages in turn, each streaming them
+// through its own cp.async ring, and merge at the end. Splits meet in a second kernel, in split order.
 //
-// Quantized pages are half the bytes of BF16 ones, so the same HBM rate brings twice the keys; the
-// codes become FP16 exactly in registers (cvt.rn.f16x2.e4m3x2):
-// - Q is scaled a row by a power of two (exact) so that FP16 holds it; S = Q K^T * (k scale * ...).
-// - V's scales join the exponent: with w_j = log2(v scale of j), the weights exp2(s_j + w_j - m) of
-//   the codes have their own running maximum m of s + w, so FP16 (scaled by 2^14) holds them with
-//   an underflow of 2^-38 of the largest; the sum of probabilities adds each weight / v scale.
+// Keys are the MMA's M (a page's 16) and query rows its N (8 a tile), so few rows waste little:
+// S^T = K Q^T, and O^T = V^T P^T with P^T from S^T by movmatrix. A decode row of eight heads a
+// key/value head takes half of the products and accumulators of the form with rows as M.
+//
+// Quantized pages are half the bytes of BF16 ones, so the same HBM rate brings twice the keys; what
+// the warps issue a page decides. The codes become FP16 exactly in registers (cvt.rn.f16x2.e4m3x2):
+// - Q is scaled a row by a power of two (exact) so that FP16 holds it; K's scales multiply S.
+// - V's scales multiply the weights before they round to FP16, by way of a power of two that keeps
+//   the largest scale seen near one; that and the rows' maxima move only when a page exceeds them
+//   (the maxima by 2^4), which one vote a page finds. Weights stay below 2^15 of FP16's 65504 and
+//   lose what lies 2^-34 below the largest.
 // - K fragments are read 16 codes a lane: the MMA's k index runs over the head's elements in the
 //   order that makes each lane's codes contiguous (Q's fragments follow the same order). V
 //   fragments come from ldmatrix.trans over byte pairs, one prmt apart.
 // Sums and statistics are FP32; P rounds to FP16 (BF16 over a BF16 cache), o once to BF16.
-
-#include <cfloat>
 
 #include "decode_ops.cuh"
 #include "launch.cuh"
@@ -32,7 +35,8 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWarps = 4;
-constexpr float kLift = 14.f;  // weights are scaled by 2^14 (at most 2^14 of FP16's 65504)
+constexpr float kLift = 10.f;   // weights are scaled by 2^10 ...
+constexpr float kSlack = 4.f;   // ... and may exceed the row's reference maximum by 2^4
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -101,9 +105,11 @@ __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
 }
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
-  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+// Transposes the warp's 8 x 8 matrix of 16-bit values (row g, columns 2t and 2t + 1 a lane).
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 
 // Layout of one 16-key page of K or V in shared memory: rows of kRow bytes in 16-byte chunks, XOR
@@ -124,12 +130,6 @@ struct Page {
   }
 };
 
-struct Item {  // what a CTA works on
-  Segment seg;
-  int kvh, m0, split;
-  bool ok;  // the segment's fields fit the launch
-};
-
 // Whether the segment's rows lie in q, and whether all of it fits the launch's sizes.
 __device__ __forceinline__ bool rows_fit(const TreeAttention& p, const Segment& s) {
   return s.row_start >= 0 && s.len > 0 && (long)s.row_start + s.len <= p.rows;
@@ -148,13 +148,21 @@ __device__ __forceinline__ bool sees(const TreeAttention& p, const Segment& s, i
 }
 
 // ------------------------------------------------------------------------------------ main kernel
-template <int D, bool kQ, int kStages>
-__global__ void __launch_bounds__(32 * kWarps, kQ ? 3 : 2)
+template <int D, bool kQ, int NT>
+struct Shape {
+  static constexpr int kStages = kQ ? 3 : 2;
+  static constexpr int kCtas = NT == 1 ? (kQ ? 4 : 3) : 2;  // of an SM, by registers and shared memory
+  static constexpr int kSmem = kWarps * kStages * 2 * Page<D, kQ>::kBytes;
+};
+
+template <int D, bool kQ, int NT>
+__global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
     tree_attention_kernel(const TreeAttention p, int mtiles, int max_splits) {
   using P = Page<D, kQ>;
+  constexpr int kStages = Shape<D, kQ, NT>::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr int kSteps = D / 16;   // 16-wide k-steps of Q K^T
-  constexpr int kNt = D / 8;       // 8-wide column tiles of O
+  constexpr int kSteps = D / 16;  // 16-wide k-steps of K Q^T, and 16-row tiles of O^T
+  constexpr int kRows = 8 * NT;
   const int G = p.q_heads / p.kv_heads;
   int item = blockIdx.x;
   const int mt = item % mtiles;
@@ -179,31 +187,77 @@ __global__ void __launch_bounds__(32 * kWarps, kQ ? 3 : 2)
     return;
   }
   const int M = seg.len * G;
-  const int m0 = mt * 16;
+  const int m0 = mt * kRows;
   const int keys = seg.cached + seg.len;
   const int nsplit = (keys + p.keys_per_split - 1) / p.keys_per_split;
   if (m0 >= M || split >= nsplit) return;
   const int k0 = split * p.keys_per_split;
   const int k1 = min(keys, k0 + p.keys_per_split);
 
-  // Q fragments of rows m0 + g and m0 + g + 8 (zeros past M). k-step s of the quantized form takes
-  // of lane t the elements 16 (t + 4 h) + 4 i .. + 3 with s = 4 h + i.
-  uint32_t qa[kSteps][4];
-  float qscale[2];
-  const int row0 = m0 + g, row1 = m0 + g + 8;
-  const int tok0 = row0 / G, tok1 = row1 / G;
+  const uint32_t wbase = smem_u32(smem) + warp * kStages * 2 * P::kBytes;
+  const uint8_t* cache = static_cast<const uint8_t*>(p.cache);
+  const int32_t* table = p.table + seg.table_start;
+  const int b_last = (k1 - 1) / 16;
+  const int b_first = k0 / 16 + warp;  // this warp's pages: b_first, b_first + kWarps, ...
+  // Block IDs of 32 of the warp's pages, one a lane.
+  int ids = 0, ids_at = b_first;
+  if (b_first + lane * kWarps <= b_last) ids = table[b_first + lane * kWarps];
+
+  auto issue = [&](int b, int stage) {
+    if (b >= ids_at + 32 * kWarps) {
+      ids_at = b;
+      if (b + lane * kWarps <= b_last) ids = table[b + lane * kWarps];
+    }
+    int id = __shfl_sync(0xffffffffu, ids, (b - ids_at) / kWarps);
+    // A block ID outside the cache reads zeros and records the bad index.
+    const bool valid = id >= 0 && id < p.cache_blocks;
+    if (!valid) {
+      if (lane == 0) record_status(p.status, kBadIndex);
+      id = 0;
+    }
+    const uint8_t* kp = cache + ((long)id * 2 * p.kv_heads + kvh) * P::kBytes + lane * 16;
+    const uint8_t* vp = kp + (long)p.kv_heads * P::kBytes;
+    const uint32_t kt = wbase + stage * 2 * P::kBytes, vt = kt + P::kBytes;
+    const int n = valid ? 16 : 0;
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int m = r ? row1 : row0;
+    for (int i = 0; i < (16 * P::kChunks) / 32; ++i) {
+      const int chunk = lane + i * 32;
+      const uint32_t dst = P::at(chunk / P::kChunks, chunk % P::kChunks);
+      cp_async16(kt + dst, kp + i * 512, n);
+      cp_async16(vt + dst, vp + i * 512, n);
+    }
+    if constexpr (kQ) {
+      if (lane < 4) {
+        cp_async16(kt + P::kCodes + lane * 16, kp + P::kCodes, n);
+        cp_async16(vt + P::kCodes + lane * 16, vp + P::kCodes, n);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    if (b_first + i * kWarps <= b_last)
+      issue(b_first + i * kWarps, i);
+    else
+      cp_async_commit();
+  }
+
+  // Q fragments: column g of tile n is row m0 + 8 n + g (zeros past M). k-step s of the quantized
+  // form takes of lane t the elements 16 (t + 4 h) + 4 i .. + 3 with s = 4 h + i.
+  uint32_t qb[NT][kSteps][2];
+  float c_[NT][2];  // scale to log2 units of this lane's columns 2t, 2t + 1
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int m = m0 + 8 * n + g;
     const __nv_bfloat16* src =
         m < M ? p.q + (long)(seg.row_start + m / G) * p.ld_q + (long)(kvh * G + m % G) * D : nullptr;
-    // Each lane's elements: D / 4 of the row in 8-byte pieces, in the order of the k-steps.
     uint2 raw[kSteps];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const int e = kQ ? 16 * (t + 4 * (s >> 2)) + 4 * (s & 3) : 8 * (t + 4 * (s >> 1)) + 4 * (s & 1);
       raw[s] = src != nullptr ? *reinterpret_cast<const uint2*>(src + e) : make_uint2(0u, 0u);
     }
+    float c = p.scale * kLog2e;
     if constexpr (kQ) {
       float amax = 0.f;
 #pragma unroll
@@ -215,72 +269,42 @@ __global__ void __launch_bounds__(32 * kWarps, kQ ? 3 : 2)
       // 2^-38 below the row's largest.
       const int e = min(max((int)(__float_as_uint(amax) >> 23), 15), 254) - 127;
       const float down = __uint_as_float((uint32_t)(127 + 14 - e) << 23);  // 14 - e in [-113, 126]
-      qscale[r] = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+      c *= __uint_as_float((uint32_t)(127 - 14 + e) << 23);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        qa[s][r] = pack_f16x2(bf16_lo(raw[s].x) * down, bf16_hi(raw[s].x) * down);
-        qa[s][r + 2] = pack_f16x2(bf16_lo(raw[s].y) * down, bf16_hi(raw[s].y) * down);
+        qb[n][s][0] = pack_f16x2(bf16_lo(raw[s].x) * down, bf16_hi(raw[s].x) * down);
+        qb[n][s][1] = pack_f16x2(bf16_lo(raw[s].y) * down, bf16_hi(raw[s].y) * down);
       }
     } else {
-      qscale[r] = 1.f;
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        qa[s][r] = raw[s].x;
-        qa[s][r + 2] = raw[s].y;
+        qb[n][s][0] = raw[s].x;
+        qb[n][s][1] = raw[s].y;
       }
     }
+    c_[n][0] = __shfl_sync(0xffffffffu, c, 8 * t);
+    c_[n][1] = __shfl_sync(0xffffffffu, c, 8 * t + 4);
   }
-  const float c0 = p.scale * kLog2e * qscale[0], c1 = p.scale * kLog2e * qscale[1];
 
-  float o[kNt][4];
+  // O^T: tile c, entries (row, column) = (g, 2t), (g, 2t + 1), (g + 8, 2t), (g + 8, 2t + 1).
+  float o[NT][kSteps][4];
+  float m_[NT][2], l_[NT][2];
 #pragma unroll
-  for (int j = 0; j < kNt; ++j)
+  for (int n = 0; n < NT; ++n) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
-  float m_[2] = {-INFINITY, -INFINITY}, l_[2] = {0.f, 0.f};
-
-  const uint32_t wbase = smem_u32(smem) + warp * kStages * 2 * P::kBytes;
-  const long page = (long)P::kBytes;
-  const uint8_t* cache = static_cast<const uint8_t*>(p.cache);
-  const int b_first = k0 / 16, b_last = (k1 - 1) / 16;
-  const int32_t* table = p.table + seg.table_start;
-
-  auto issue = [&](int b, int stage) {
-    int id = table[b];
-    // A block ID outside the cache reads zeros and records the bad index.
-    const bool valid = id >= 0 && id < p.cache_blocks;
-    if (!valid) {
-      if (lane == 0) record_status(p.status, kBadIndex);
-      id = 0;
-    }
-    const uint8_t* kp = cache + ((long)id * 2 * p.kv_heads + kvh) * page;
-    const uint8_t* vp = kp + (long)p.kv_heads * page;
-    const uint32_t kt = wbase + stage * 2 * P::kBytes, vt = kt + P::kBytes;
+    for (int c = 0; c < kSteps; ++c)
 #pragma unroll
-    for (int i = 0; i < (16 * P::kChunks) / 32; ++i) {
-      const int chunk = lane + i * 32;
-      const uint32_t dst = P::at(chunk / P::kChunks, chunk % P::kChunks);
-      cp_async16(kt + dst, kp + chunk * 16, valid ? 16 : 0);
-      cp_async16(vt + dst, vp + chunk * 16, valid ? 16 : 0);
-    }
-    if constexpr (kQ) {
-      if (lane < 8)
-        cp_async16((lane < 4 ? kt : vt) + P::kCodes + (lane & 3) * 16, (lane < 4 ? kp : vp) + P::kCodes + (lane & 3) * 16,
-                   valid ? 16 : 0);
-    }
-    cp_async_commit();
-  };
-
-  int b = b_first + warp;
-  bool odd_v = false;  // this warp left values that are not finite out of the products
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) {
-    if (b + i * kWarps <= b_last)
-      issue(b + i * kWarps, i);
-    else
-      cp_async_commit();
+      for (int i = 0; i < 4; ++i) o[n][c][i] = 0.f;
+    m_[n][0] = m_[n][1] = -INFINITY;
+    l_[n][0] = l_[n][1] = 0.f;
   }
-  for (int stage = 0; b <= b_last; b += kWarps, stage = stage + 1 == kStages ? 0 : stage + 1) {
+  int v_exp = -126;            // exponent of the largest V scale of the pages so far
+  float v_inv = 0x1p126f;      // 2^-v_exp
+  float v_lim = 0x1p-125f;     // 2^(v_exp + 1)
+  bool odd_v = false;          // this lane left values that are not finite out of the products
+
+  int stage = 0;
+  for (int b = b_first; b <= b_last; b += kWarps, stage = stage + 1 == kStages ? 0 : stage + 1) {
     const int ahead = b + (kStages - 1) * kWarps;
     if (ahead <= b_last)
       issue(ahead, stage == 0 ? kStages - 1 : stage - 1);
@@ -300,7 +324,7 @@ __global__ void __launch_bounds__(32 * kWarps, kQ ? 3 : 2)
         if (key < seg.cached) continue;
         const uint32_t a = vt + P::at(chunk / P::kChunks, chunk % P::kChunks);
         uint4 v = lds128(a);
-        uint32_t* w = &v.x;
+        uint32_t w[4] = {v.x, v.y, v.z, v.w};
         bool change = false;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -320,218 +344,256 @@ __global__ void __launch_bounds__(32 * kWarps, kQ ? 3 : 2)
             w[e] &= ~bad;
           }
         }
-        if (change) sts128(a, v);
+        if (change) sts128(a, make_uint4(w[0], w[1], w[2], w[3]));
       }
       __syncwarp();
     }
 
-    // S = Q K^T of the page's two 8-key tiles.
-    float s[2][4];
+    // S^T of the page: rows are keys g and g + 8.
+    float s[NT][4];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
-      if constexpr (kQ) {
+    if constexpr (kQ) {
 #pragma unroll
-        for (int h = 0; h < kSteps / 4; ++h) {
-          const uint4 w = lds128(kt + P::at(n * 8 + g, t + 4 * h));
-          mma_f16(s[n], qa[4 * h], e4m3x2_f16x2(w.x), e4m3x2_f16x2_hi(w.x));
-          mma_f16(s[n], qa[4 * h + 1], e4m3x2_f16x2(w.y), e4m3x2_f16x2_hi(w.y));
-          mma_f16(s[n], qa[4 * h + 2], e4m3x2_f16x2(w.z), e4m3x2_f16x2_hi(w.z));
-          mma_f16(s[n], qa[4 * h + 3], e4m3x2_f16x2(w.w), e4m3x2_f16x2_hi(w.w));
+      for (int h = 0; h < kSteps / 4; ++h) {
+        const uint4 x = lds128(kt + P::at(g, t + 4 * h)), y = lds128(kt + P::at(g + 8, t + 4 * h));
+        const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t a[4] = {e4m3x2_f16x2(xw[i]), e4m3x2_f16x2(yw[i]), e4m3x2_f16x2_hi(xw[i]), e4m3x2_f16x2_hi(yw[i])};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16(s[n], a, qb[n][4 * h + i][0], qb[n][4 * h + i][1]);
         }
-      } else {
+      }
+    } else {
 #pragma unroll
-        for (int h = 0; h < kSteps / 2; ++h) {
-          const uint4 w = lds128(kt + P::at(n * 8 + g, t + 4 * h));
-          mma_b16(s[n], qa[2 * h], w.x, w.y);
-          mma_b16(s[n], qa[2 * h + 1], w.z, w.w);
+      for (int h = 0; h < kSteps / 2; ++h) {
+        const uint4 x = lds128(kt + P::at(g, t + 4 * h)), y = lds128(kt + P::at(g + 8, t + 4 * h));
+        const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma_b16(s[n], a0, qb[n][2 * h][0], qb[n][2 * h][1]);
+          mma_b16(s[n], a1, qb[n][2 * h + 1][0], qb[n][2 * h + 1][1]);
         }
       }
     }
 
-    // Scaled scores (log2 units) with V's exponents, masked; the rows' maxima.
-    float inv_v[2][2];  // 1 / v scale of this lane's keys
+    // Scores in log2 units; masked ones are -inf.
+    float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
+    if constexpr (kQ) {
+      ks[0] = lds_f32(kt + P::kCodes + g * 4);
+      ks[1] = lds_f32(kt + P::kCodes + g * 4 + 32);
+      vs[0] = lds_f32(vt + P::kCodes + g * 4);
+      vs[1] = lds_f32(vt + P::kCodes + g * 4 + 32);
+    }
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float ks = 1.f, w = 0.f;
-        inv_v[n][i] = 1.f;
-        if constexpr (kQ) {
-          ks = lds_f32(kt + P::kCodes + (n * 8 + 2 * t + i) * 4);
-          const float vs = lds_f32(vt + P::kCodes + (n * 8 + 2 * t + i) * 4);
-          if (vs > 0.f) {  // (a page of zeros has zero scales, whose codes are zeros too)
-            w = __log2f(vs);
-            inv_v[n][i] = __fdividef(1.f, vs);
-          }
-        }
-        s[n][i] = fmaf(s[n][i], c0 * ks, w);
-        s[n][i + 2] = fmaf(s[n][i + 2], c1 * ks, w);
-      }
+      for (int i = 0; i < 4; ++i) s[n][i] *= kQ ? c_[n][i & 1] * ks[i >> 1] : c_[n][i & 1];
     if (!inner) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int r = 0; r < 2; ++r) {
+        const int key = b * 16 + g + 8 * r;
+        const int j = key - seg.cached;
+        if (key >= k1) vs[r] = 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int m = m0 + 8 * n + 2 * t + i;
+            if (key >= k1 || (j >= 0 && (m >= M || !sees(p, seg, m / G, j)))) s[n][2 * r + i] = -INFINITY;
+          }
+      }
+    }
+    // One vote finds whether a row's maximum or V's reference scale must move.
+    bool move = kQ && (vs[0] >= v_lim || vs[1] >= v_lim);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) move = move || fmaxf(s[n][i], s[n][i + 2]) > m_[n][i] + kSlack;
+    if (__any_sync(0xffffffffu, move)) {
+      float fv = 1.f;
+      if constexpr (kQ) {
+        // (Scales are not negative: their bits order as they do.)
+        const uint32_t top = __reduce_max_sync(0xffffffffu, max(__float_as_uint(fmaxf(vs[0], 0.f)), __float_as_uint(fmaxf(vs[1], 0.f))));
+        const int e = max(v_exp, min(max((int)(top >> 23), 1), 253) - 127);
+        fv = ex2((float)(v_exp - e));
+        v_exp = e;
+        v_inv = __uint_as_float((uint32_t)(127 - e) << 23);  // e <= 126
+        v_lim = __uint_as_float((uint32_t)(128 + e) << 23);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int key = b * 16 + n * 8 + 2 * t + i;
-          const int j = key - seg.cached;
-          if (key >= k1) inv_v[n][i] = 0.f;
-          if (key >= k1 || (j >= 0 && (row0 >= M || !sees(p, seg, tok0, j)))) s[n][i] = -INFINITY;
-          if (key >= k1 || (j >= 0 && (row1 >= M || !sees(p, seg, tok1, j)))) s[n][i + 2] = -INFINITY;
+          float x = fmaxf(s[n][i], s[n][i + 2]);
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(m_[n][i], fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16)));
+          // A row with no visible key yet keeps a zero state.
+          const float f = x == -INFINITY ? 1.f : ex2(m_[n][i] - x);
+          m_[n][i] = x;
+          l_[n][i] *= f;
+#pragma unroll
+          for (int c = 0; c < kSteps; ++c) {
+            o[n][c][i] *= f * fv;
+            o[n][c][i + 2] *= f * fv;
+          }
         }
     }
-    float n0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-    float n1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
-    n0 = fmaxf(m_[0], quad_max(n0));
-    n1 = fmaxf(m_[1], quad_max(n1));
-    // A row with no visible key yet keeps a zero state.
-    const float f0 = n0 == -INFINITY ? 1.f : ex2(m_[0] - n0);
-    const float f1 = n1 == -INFINITY ? 1.f : ex2(m_[1] - n1);
-    const float z0 = n0 == -INFINITY ? 0.f : n0 - kLift, z1 = n1 == -INFINITY ? 0.f : n1 - kLift;
-    m_[0] = n0;
-    m_[1] = n1;
-    float sum0 = 0.f, sum1 = 0.f;
+
+    // Weights, their sums, and P^T as the B operand (rows are keys).
+    uint32_t pb[NT][2];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < NT; ++n) {
+      float w[4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        s[n][i] = ex2(s[n][i] - z0);
-        s[n][i + 2] = ex2(s[n][i + 2] - z1);
-        sum0 = fmaf(s[n][i], inv_v[n][i], sum0);
-        sum1 = fmaf(s[n][i + 2], inv_v[n][i], sum1);
+      for (int i = 0; i < 4; ++i) {
+        const float z = m_[n][i & 1] == -INFINITY ? 0.f : m_[n][i & 1] - kLift;
+        w[i] = ex2(s[n][i] - z);
+        l_[n][i & 1] += w[i];
+        if constexpr (kQ) w[i] *= vs[i >> 1] * v_inv;
       }
-    l_[0] = l_[0] * f0 + sum0;
-    l_[1] = l_[1] * f1 + sum1;
-    if (__any_sync(0xffffffffu, f0 != 1.f || f1 != 1.f)) {
-#pragma unroll
-      for (int j = 0; j < kNt; ++j) {
-        o[j][0] *= f0;
-        o[j][1] *= f0;
-        o[j][2] *= f1;
-        o[j][3] *= f1;
+      if constexpr (kQ) {
+        pb[n][0] = transpose8(pack_f16x2(w[0], w[1]));
+        pb[n][1] = transpose8(pack_f16x2(w[2], w[3]));
+      } else {
+        pb[n][0] = transpose8(pack_bf16x2(w[0], w[1]));
+        pb[n][1] = transpose8(pack_bf16x2(w[2], w[3]));
       }
     }
 
-    // O += P V: the 16 keys are one k-step.
-    uint32_t pa[4];
+    // O^T += V^T P^T.
     if constexpr (kQ) {
-      pa[0] = pack_f16x2(s[0][0], s[0][1]);
-      pa[1] = pack_f16x2(s[0][2], s[0][3]);
-      pa[2] = pack_f16x2(s[1][0], s[1][1]);
-      pa[3] = pack_f16x2(s[1][2], s[1][3]);
-    } else {
-      pa[0] = pack_bf16x2(s[0][0], s[0][1]);
-      pa[1] = pack_bf16x2(s[0][2], s[0][3]);
-      pa[2] = pack_bf16x2(s[1][0], s[1][1]);
-      pa[3] = pack_bf16x2(s[1][2], s[1][3]);
-    }
-    // ldmatrix.trans: lanes 0-7 keys 0-7 chunk c, 8-15 keys 8-15 chunk c, 16-31 the same of c + 1.
+      // ldmatrix.trans: lanes 0-7 keys 0-7 chunk c, 8-15 keys 8-15 chunk c, 16-31 the same of c + 1.
+      // A register holds (two keys) x (two neighbouring elements): prmt makes them (two elements)
+      // x (two keys). A tile's rows 0-7 are a chunk's even elements, 8-15 its odd ones.
 #pragma unroll
-    for (int c = 0; c < P::kChunks; c += 2) {
-      uint32_t r[4];
-      ldsm_x4_t(r, vt + P::at(lane & 15, c + (lane >> 4)));
-      if constexpr (kQ) {
-        // A register holds (two keys) x (two neighbouring elements): prmt makes them (two elements)
-        // x (two keys). Tile 2c takes a chunk's even elements, 2c + 1 its odd ones.
+      for (int c = 0; c < P::kChunks; c += 2) {
+        uint32_t r[4];
+        ldsm_x4_t(r, vt + P::at(lane & 15, c + (lane >> 4)));
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           const uint32_t lo = __byte_perm(r[2 * w], 0u, 0x3120), hi = __byte_perm(r[2 * w + 1], 0u, 0x3120);
-          mma_f16(o[2 * (c + w)], pa, e4m3x2_f16x2(lo), e4m3x2_f16x2(hi));
-          mma_f16(o[2 * (c + w) + 1], pa, e4m3x2_f16x2_hi(lo), e4m3x2_f16x2_hi(hi));
+          const uint32_t a[4] = {e4m3x2_f16x2(lo), e4m3x2_f16x2_hi(lo), e4m3x2_f16x2(hi), e4m3x2_f16x2_hi(hi)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16(o[n][c + w], a, pb[n][0], pb[n][1]);
         }
-      } else {
-        mma_b16(o[c], pa, r[0], r[1]);
-        mma_b16(o[c + 1], pa, r[2], r[3]);
+      }
+    } else {
+      // ldmatrix.trans: lanes 0-15 keys 0-7 of chunks 2c and 2c + 1, 16-31 keys 8-15 of them.
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) {
+        uint32_t r[4];
+        ldsm_x4_t(r, vt + P::at((lane & 7) + 8 * (lane >> 4), 2 * c + (lane >> 3 & 1)));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_b16(o[n][c], r, pb[n][0], pb[n][1]);
       }
     }
     __syncwarp();
   }
 
   // Merge the warps: row statistics, then the rescaled sums, through shared memory.
-  l_[0] = quad_sum(l_[0]);
-  l_[1] = quad_sum(l_[1]);
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l_[n][i] += __shfl_xor_sync(0xffffffffu, l_[n][i], x);
   cp_async_wait<0>();
   __syncthreads();  // every warp is done with its pages
-  float* sm_m = reinterpret_cast<float*>(smem);  // [kWarps][16]
-  float* sm_l = sm_m + 16 * kWarps;
-  float* sm_o = sm_l + 16 * kWarps;  // [16][D]
-  if (t == 0) {
-    sm_m[warp * 16 + g] = m_[0];
-    sm_m[warp * 16 + g + 8] = m_[1];
-    sm_l[warp * 16 + g] = l_[0];
-    sm_l[warp * 16 + g + 8] = l_[1];
+  float* sm_m = reinterpret_cast<float*>(smem);  // [kWarps][kRows]
+  float* sm_l = sm_m + kRows * kWarps;
+  float* sm_o = sm_l + kRows * kWarps;  // [kWarps][kRows][D]
+  static_assert((2 * 16 * kWarps + kWarps * 16 * D) * 4 <= Shape<D, kQ, 2>::kSmem, "merge fits the ring");
+  static_assert((2 * 8 * kWarps + kWarps * 8 * D) * 4 <= Shape<D, kQ, 1>::kSmem, "merge fits the ring");
+  if (g == 0) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        sm_m[warp * kRows + 8 * n + 2 * t + i] = m_[n][i];
+        sm_l[warp * kRows + 8 * n + 2 * t + i] = l_[n][i];
+      }
   }
-  const bool fix = __syncthreads_or(odd_v);
-  float top[2], w_[2];
+  const float back = kQ ? __uint_as_float((uint32_t)(127 + v_exp) << 23) : 1.f;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float mm = -INFINITY;
-    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sm_m[w * 16 + g + 8 * h]);
-    top[h] = mm;
-    w_[h] = m_[h] == -INFINITY ? 0.f : ex2(m_[h] - mm);
-  }
-  for (int w = 0; w < kWarps; ++w) {
-    if (warp == w) {
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int j = 0; j < kNt; ++j)
+    for (int i = 0; i < 2; ++i) {
+      float* dst = sm_o + (warp * kRows + 8 * n + 2 * t + i) * D;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int c = kQ ? 16 * (j >> 1) + 4 * t + 2 * i + (j & 1) : j * 8 + 2 * t + i;
-            float* dst = sm_o + (g + 8 * h) * D + c;
-            const float v = o[j][2 * h + i] * w_[h];
-            *dst = w == 0 ? v : *dst + v;
-          }
+      for (int c = 0; c < kSteps; ++c) {
+        if constexpr (kQ) {
+          *reinterpret_cast<float2*>(dst + 16 * c + 2 * g) = make_float2(o[n][c][i] * back, o[n][c][i + 2] * back);
+        } else {
+          dst[16 * c + g] = o[n][c][i];
+          dst[16 * c + g + 8] = o[n][c][i + 2];
+        }
+      }
     }
-    __syncthreads();
-  }
-  const int rows = min(16, M - m0);
-  for (int i = threadIdx.x; i < rows * D; i += 32 * kWarps) {
-    const int r = i / D, c = i % D;
+  const bool fix = __syncthreads_or(odd_v);
+  const int rows = min(kRows, M - m0);
+  for (int i = threadIdx.x; i < rows * (D / 2); i += 32 * kWarps) {
+    const int r = i / (D / 2), c = 2 * (i % (D / 2));
     const int m = m0 + r, tok = m / G, head = kvh * G + m % G;
     float mm = -INFINITY, ll = 0.f;
-    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sm_m[w * 16 + r]);
+    float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sm_m[w * kRows + r]);
+#pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float mw = sm_m[w * 16 + r];
-      ll += mw == -INFINITY ? 0.f : sm_l[w * 16 + r] * ex2(mw - mm);
+      const float mw = sm_m[w * kRows + r];
+      const float f = mw == -INFINITY ? 0.f : ex2(mw - mm);
+      const float2 x = *reinterpret_cast<const float2*>(sm_o + (w * kRows + r) * D + c);
+      ll = fmaf(f, sm_l[w * kRows + r], ll);
+      v.x = fmaf(f, x.x, v.x);
+      v.y = fmaf(f, x.y, v.y);
     }
-    float v = sm_o[i];
     if (fix) {
       for (int j = max(0, k0 - seg.cached); j < min(seg.len, k1 - seg.cached); ++j) {
         if (!sees(p, seg, tok, j)) continue;
         const int key = seg.cached + j, id = table[key >> 4];
         if (id < 0 || id >= p.cache_blocks) continue;
-        const uint8_t* vp = cache + ((long)id * 2 * p.kv_heads + p.kv_heads + kvh) * page + (key & 15) * P::kRow;
+        const uint8_t* vp = cache + ((long)id * 2 * p.kv_heads + p.kv_heads + kvh) * P::kBytes + (key & 15) * P::kRow;
         if constexpr (kQ) {
-          if ((vp[c] & 0x7fu) == 0x7fu) v = __int_as_float(0x7fffffff);
+          if ((vp[c] & 0x7fu) == 0x7fu) v.x = __int_as_float(0x7fffffff);
+          if ((vp[c + 1] & 0x7fu) == 0x7fu) v.y = __int_as_float(0x7fffffff);
         } else {
           const float x = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(vp)[c]);
-          if (!(fabsf(x) < INFINITY)) v += x;
+          const float y = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(vp)[c + 1]);
+          if (!(fabsf(x) < INFINITY)) v.x += x;
+          if (!(fabsf(y) < INFINITY)) v.y += y;
         }
       }
     }
     const long at = (long)(seg.row_start + tok);
     if (nsplit == 1) {
-      p.o[at * p.ld_o + (long)head * D + c] = __float2bfloat16_rn(mm == -INFINITY ? 0.f : v / ll);
+      const float inv = mm == -INFINITY ? 0.f : 1.f / ll;
+      *reinterpret_cast<uint32_t*>(p.o + at * p.ld_o + (long)head * D + c) = pack_bf16x2(v.x * inv, v.y * inv);
     } else {
       const long idx = (at * p.q_heads + head) * max_splits + split;
-      p.partial_o[idx * D + c] = v;
+      *reinterpret_cast<float2*>(p.partial_o + idx * D + c) = v;
       if (c == 0) p.partial_ml[idx] = make_float2(mm, ll);
     }
   }
 }
 
-// Joins the splits of each (row, head), in split order: one warp each.
+// Joins the splits of each (row, head): a CTA each, whose warps take the splits in turn and meet in
+// a fixed order. (One warp a head took 20 us for 64 splits of 192 heads: it waits for one load
+// after another.)
 template <int D>
-__global__ void __launch_bounds__(256) tree_merge_kernel(const TreeAttention p, int max_splits) {
+__global__ void __launch_bounds__(128) tree_merge_kernel(const TreeAttention p, int max_splits) {
+  constexpr int E = D / 32;
+  __shared__ float sm_acc[3][D], sm_den[3];
   pdl_wait();
   pdl_trigger();
   const Segment seg = p.segments[blockIdx.x / p.max_len];
   const int tok = blockIdx.x % p.max_len;
-  const int head = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (tok >= seg.len || head >= p.q_heads || !rows_fit(p, seg) || !segment_fits(p, seg)) return;
+  const int head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (tok >= seg.len || !rows_fit(p, seg) || !segment_fits(p, seg)) return;
   const int nsplit = (seg.cached + seg.len + p.keys_per_split - 1) / p.keys_per_split;
   if (nsplit == 1) return;  // written in place
   const long row = seg.row_start + tok;
@@ -540,51 +602,81 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeAttention p, 
   for (int s = lane; s < nsplit; s += 32) top = fmaxf(top, p.partial_ml[base + s].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  constexpr int E = D / 32;
   float acc[E], den = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
   if (top > -INFINITY) {
 #pragma unroll 4
-    for (int s = 0; s < nsplit; ++s) {
+    for (int s = warp; s < nsplit; s += 4) {
       const float2 ml = p.partial_ml[base + s];
       const float w = ex2(ml.x - top);
       den = fmaf(w, ml.y, den);
       const float* src = p.partial_o + (base + s) * D + lane * E;
+      float x[E];
+      if constexpr (E == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(src);
+        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+      } else {
+        const float2 v = *reinterpret_cast<const float2*>(src);
+        x[0] = v.x, x[1] = v.y;
+      }
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = fmaf(w, src[e], acc[e]);
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(w, x[e], acc[e]);
     }
-  } else {
-    den = 1.f;
+  }
+  if (warp > 0) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) sm_acc[warp - 1][lane * E + e] = acc[e];
+    if (lane == 0) sm_den[warp - 1] = den;
+  }
+  __syncthreads();
+  if (warp > 0) return;
+#pragma unroll
+  for (int w = 0; w < 3; ++w) {
+    den += sm_den[w];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] += sm_acc[w][lane * E + e];
   }
   __nv_bfloat16* dst = p.o + row * p.ld_o + (long)head * D + lane * E;
-  const float inv = 1.f / den;
+  const float inv = top > -INFINITY ? 1.f / den : 0.f;
 #pragma unroll
   for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
 }
 
-template <int D, bool kQ>
+template <int D>
+int merge(const TreeAttention& p, int splits, cudaStream_t stream) {
+  if (splits == 1) return 0;
+  return launch_pdl(tree_merge_kernel<D>, dim3(p.num_segments * p.max_len, p.q_heads), dim3(128), 0, stream, p, splits) ==
+                 cudaSuccess
+             ? 0
+             : -5;
+}
+
+template <int D, bool kQ, int NT>
 int launch(const TreeAttention& p, cudaStream_t stream) {
-  constexpr int kStages = kQ ? 4 : 3;
   const int G = p.q_heads / p.kv_heads;
-  const int splits = (p.max_keys + p.keys_per_split - 1) / p.keys_per_split;
-  if (splits > 65535) return -2;
-  if (splits > 1) {
-    const size_t need = (size_t)p.rows * p.q_heads * splits;
-    if (p.partial_o == nullptr || p.partial_ml == nullptr || need > p.partial_capacity) return -3;
-  }
-  const long mtiles = ((long)p.max_len * G + 15) / 16;
+  const int splits = ((long)p.max_keys + p.keys_per_split - 1) / p.keys_per_split;
+  const long mtiles = ((long)p.max_len * G + 8 * NT - 1) / (8 * NT);
   const long ctas = mtiles * p.kv_heads * p.num_segments;
-  if (ctas > 2147483647L || (long)p.num_segments * p.max_len > 2147483647L) return -2;
-  constexpr int smem = kWarps * kStages * 2 * Page<D, kQ>::kBytes;
-  const auto kernel = tree_attention_kernel<D, kQ, kStages>;
+  if (ctas > 2147483647L) return -2;
+  constexpr int smem = Shape<D, kQ, NT>::kSmem;
+  const auto kernel = tree_attention_kernel<D, kQ, NT>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -5;
   if (launch_pdl(kernel, dim3((unsigned)ctas, splits), dim3(32 * kWarps), smem, stream, p, (int)mtiles, splits) != cudaSuccess)
     return -5;
-  if (splits > 1 && launch_pdl(tree_merge_kernel<D>, dim3(p.num_segments * p.max_len, (p.q_heads + 7) / 8), dim3(256), 0,
-                               stream, p, splits) != cudaSuccess)
-    return -5;
-  return 0;
+  return merge<D>(p, splits, stream);
+}
+
+// Whether a segment may have more rows than the mma.sync form holds in one tile.
+bool tc_rows(int max_len, int group) { return (long)max_len * group > 16; }
+
+template <int D, bool kQ>
+int pick(const TreeAttention& p, cudaStream_t stream) {
+  if (tc_rows(p.max_len, p.q_heads / p.kv_heads) && tree_attention_tc_supported(p)) {
+    const int rc = tree_attention_tc(p, stream);
+    return rc != 0 ? rc : merge<D>(p, (p.max_keys + p.keys_per_split - 1) / p.keys_per_split, stream);
+  }
+  return (long)p.max_len * (p.q_heads / p.kv_heads) <= 8 ? launch<D, kQ, 1>(p, stream) : launch<D, kQ, 2>(p, stream);
 }
 
 }  // namespace
@@ -592,13 +684,16 @@ int launch(const TreeAttention& p, cudaStream_t stream) {
 int tree_attention_split(int num_segments, int q_heads, int kv_heads, int head_dim, int quantized, int max_keys,
                          int max_len) {
   if (num_segments <= 0 || kv_heads <= 0 || max_keys <= 0) return 16;
-  const long tiles = ((long)max_len * (q_heads / kv_heads) + 15) / 16;
-  const long items = tiles * kv_heads * num_segments;
-  // About four CTAs for each that the GPU holds at once, of at least 64 keys a warp.
-  const long want = 148L * 3 * 4;
-  const long per = (long)max_keys * items / want;
-  long keys = per < 256 ? 256 : per;
-  keys = (keys + 63) / 64 * 64;
+  const long rows = (long)max_len * (q_heads / kv_heads);
+  const bool tc = tc_rows(max_len, (int)(q_heads / kv_heads));
+  const long tile = tc ? 256 : 16;
+  const long items = (rows + tile - 1) / tile * kv_heads * num_segments;
+  // About two (tcgen05) or four CTAs for each that the GPU holds at once, of at least so many keys
+  // that a CTA's start and end do not count.
+  const long want = tc ? 148L * 2 : 148L * 4 * 2;
+  const long least = tc ? 512 : 256;
+  const long per = ((long)max_keys * items + want - 1) / want;
+  const long keys = ((per < least ? least : per) + 127) / 128 * 128;
   return (int)(keys > max_keys ? (max_keys + 15) / 16 * 16 : keys);
 }
 
@@ -606,11 +701,17 @@ int tree_attention(const TreeAttention& p, cudaStream_t stream) {
   if (p.num_segments <= 0 || p.rows <= 0) return 0;
   if (p.kv_heads <= 0 || p.q_heads <= 0 || p.q_heads % p.kv_heads != 0) return -2;
   if (p.max_keys <= 0 || p.max_len <= 0 || p.keys_per_split <= 0 || p.keys_per_split % 16 != 0) return -2;
+  if ((long)p.num_segments * p.max_len > 2147483647L || p.q_heads > 65535) return -2;
+  const long splits = ((long)p.max_keys + p.keys_per_split - 1) / p.keys_per_split;
+  if (splits > 65535) return -2;
+  if (splits > 1 && (p.partial_o == nullptr || p.partial_ml == nullptr ||
+                     (size_t)p.rows * p.q_heads * splits > p.partial_capacity || (reinterpret_cast<uintptr_t>(p.partial_o) & 15)))
+    return -3;
   if (p.ld_q % 8 != 0 || p.ld_o % 8 != 0) return -2;
   if ((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.o) | reinterpret_cast<uintptr_t>(p.cache)) & 15)
     return -2;
-  if (p.head_dim == 64) return p.quantized ? launch<64, true>(p, stream) : launch<64, false>(p, stream);
-  if (p.head_dim == 128) return p.quantized ? launch<128, true>(p, stream) : launch<128, false>(p, stream);
+  if (p.head_dim == 64) return p.quantized ? pick<64, true>(p, stream) : pick<64, false>(p, stream);
+  if (p.head_dim == 128) return p.quantized ? pick<128, true>(p, stream) : pick<128, false>(p, stream);
   return -2;
 }
 

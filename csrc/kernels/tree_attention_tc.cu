@@ -1,0 +1,851 @@
+// Attention of chunks and drafted token trees over the paged cache on the tcgen05 tensor cores, for
+// segments whose (token, head) rows fill an MMA tile; tree_attention.cu states the operator and
+// takes the others.
+//
+// One CTA per (segment, key/value head, 256 rows, split of the keys), 128-key tiles:
+// - Two softmax warpgroups, a thread a row, each with its own S and O in TMEM. With more than 128
+//   rows they take a row tile each and share every key tile (A); with fewer they take the key tiles
+//   in turn for the same rows (B) and join their sums at the end. So one of them works on its
+//   scores while the tensor cores work for the other.
+// - P replaces S in TMEM (16 bits, half the columns) and is the A operand of O += P V from there.
+//   One thread issues every MMA, in an order that has P_w V before the next S_w.
+// - Quantized pages: K's codes are the B operand of S as they lie in the cache (kind::f8f6f4); Q
+//   enters as two E4M3 parts, hi = e4m3(q), lo = e4m3(q - hi), of rows scaled by a power of two to
+//   [128, 256). Two parts hold BF16's 8 bits exactly; what lies below 2^-17 of the row's largest is
+//   lost. V's codes become FP16 (exactly) in shared memory, by four helper warps, since weights in
+//   E4M3 would lose a long tail of small probabilities; they write the keys' scales beside it.
+// - BF16 pages: TMA brings K and V as the MMAs read them; the helpers only clear V rows past the
+//   keys and values that are not finite.
+// - Row maxima move when a tile exceeds them by 2^4, V's reference scale when a tile's largest
+//   does (tracked by the helpers): O is rescaled in TMEM then.
+// - Every wait is bounded; a timeout records a status and every role leaves through the same end.
+//
+// Over quantized pages with 256 rows the MMAs bound it (two FP8 passes of S cost what one FP16 pass
+// does), with 128 or fewer HBM does.
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "decode_ops.cuh"
+#include "launch.cuh"
+#include "sm100.cuh"
+#include "tmap.cuh"
+
+namespace foa {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLift = 10.f;   // weights are scaled by 2^10 ...
+constexpr float kSlack = 4.f;   // ... and may exceed the row's reference maximum by 2^4
+constexpr int kTile = 128;      // rows and keys of an MMA tile
+constexpr int kThreads = 448;   // 8 softmax warps, MMA, loader, 4 helpers
+constexpr int kSlots = 4;       // key tiles whose scales are held
+
+template <int D, bool kQ>
+struct Cfg {
+  static constexpr int kHalf = kTile * 128;            // a tile's 64 16-bit columns
+  static constexpr int kTile16 = kTile * D * 2;        // a 16-bit tile
+  static constexpr int kTile8 = kTile * D;             // an 8-bit tile
+  static constexpr int kQTile = kTile16;               // (hi and lo, or BF16)
+  static constexpr int kKStages = kQ ? 3 : 2;
+  static constexpr int kKStage = kQ ? kTile8 : kTile16;
+  static constexpr int kVStages = 2;
+  static constexpr int kRaw = kQ ? 2 : 0;              // stages of V's codes
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffK = kOffQ + 2 * kQTile;
+  static constexpr int kOffV = kOffK + kKStages * kKStage;
+  static constexpr int kOffRaw = kOffV + kVStages * kTile16;
+  static constexpr int kOffScale = kOffRaw + kRaw * kTile8;       // [slots][2 (K, V)][128], then [slots][4] maxima
+  static constexpr int kOffRow = kOffScale + kSlots * (2 * kTile + 4) * 4;  // [2 (maximum, sum)][128]
+  static constexpr int kOffBar = (kOffRow + 2 * kTile * 4 + 15) / 16 * 16;
+  static constexpr int kBytes = kOffBar + 256 + 1024;  // 1 KiB of alignment slack
+  // One CTA an SM: it holds all of TMEM.
+  static constexpr int kSmem = kBytes < 120 * 1024 ? 120 * 1024 : kBytes;
+  static constexpr int kColO = 2 * kTile;              // TMEM: S0, S1, then O0, O1 (128 columns apart)
+};
+
+struct Maps {
+  CUtensorMap cache;  // codes: [pages][16][D] bytes; BF16: [pages * 16][D]
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t v) {
+  uint32_t r;
+  asm("{\n .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %1;\n cvt.rn.f16x2.e4m3x2 %0, lo;\n}" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3x2_f16x2_hi(uint32_t v) {
+  uint32_t r;
+  asm("{\n .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %1;\n cvt.rn.f16x2.e4m3x2 %0, hi;\n}" : "=r"(r) : "r"(v));
+  return r;
+}
+// Pairs of FP32 operations in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 w, {%6, %7};\n"
+      " fma.rn.f32x2 z, x, y, w;\n mov.b64 {%0, %1}, z;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32"
+      " [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+// Shared-memory descriptors: a K-major 8-bit operand in rows of `kRowBytes` (128 or 64, swizzled over
+// as many bytes), and an MN-major 16-bit one (see the prefill kernel's layout: rows of 64 elements,
+// groups of 64 `lbo` bytes apart).
+template <int kRowBytes>
+__device__ __forceinline__ uint64_t desc_k8(const void* smem) {
+  uint64_t d = (smem_u32(smem) >> 4) & 0x3FFFull;
+  d |= (uint64_t)1 << 16;
+  d |= (uint64_t)((8 * kRowBytes) >> 4) << 32;              // eight rows
+  d |= (uint64_t)1 << 46;                                   // descriptor version of sm_100
+  d |= (uint64_t)(kRowBytes == 128 ? 2 : 4) << 61;          // 128- or 64-byte swizzle
+  return d;
+}
+__device__ __forceinline__ uint64_t desc_mn16(const void* smem, uint32_t lbo, uint32_t sbo) {
+  uint64_t d = (smem_u32(smem) >> 4) & 0x3FFFull;
+  d |= (uint64_t)((lbo >> 4) & 0x3FFF) << 16;
+  d |= (uint64_t)((sbo >> 4) & 0x3FFF) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+// D[tmem] (+)= A[tmem] * B[smem]^T for 16-bit operands.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 16-byte chunk `c` of row `r` in rows of kRowBytes as TMA swizzles them.
+template <int kRowBytes>
+__device__ __forceinline__ uint32_t at8(int r, int c) {
+  return kRowBytes == 128 ? (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)) : (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+}
+// 16-byte chunk `c` (8 elements) of row `r` of a 16-bit tile: halves of 64 columns.
+__device__ __forceinline__ uint32_t at16(int r, int c) {
+  return (uint32_t)((c >> 3) * kTile * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+__device__ __forceinline__ bool rows_fit(const TreeAttention& p, const Segment& s) {
+  return s.row_start >= 0 && s.len > 0 && (long)s.row_start + s.len <= p.rows;
+}
+__device__ __forceinline__ bool segment_fits(const TreeAttention& p, const Segment& s) {
+  return s.cached >= 0 && s.len <= p.max_len && (long)s.cached + s.len <= p.max_keys && s.table_start >= 0 &&
+         s.nblocks >= 0 && (long)s.table_start + s.nblocks <= p.table_len &&
+         (long)s.nblocks * 16 >= (long)s.cached + s.len;
+}
+__device__ __forceinline__ uint32_t mask_word(const TreeAttention& p, const Segment& s, int tok, int w) {
+  if (p.mask == nullptr) {  // causal: bits 0 .. tok
+    const int n = tok + 1 - 32 * w;
+    return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1;
+  }
+  return w < p.mask_words ? p.mask[(long)(s.row_start + tok) * p.mask_words + w] : 0u;
+}
+// The keys of [key, key + 32) that row `tok` sees, below k1.
+__device__ __forceinline__ uint32_t visible(const TreeAttention& p, const Segment& s, int tok, int key, int k1) {
+  const int j = key - s.cached;  // place of the first among the appended rows
+  uint32_t v;
+  if (j <= -32) {
+    v = ~0u;
+  } else if (j < 0) {
+    v = (1u << -j) - 1 | mask_word(p, s, tok, 0) << -j;
+  } else {
+    v = mask_word(p, s, tok, j >> 5) >> (j & 31);
+    if (j & 31) v |= mask_word(p, s, tok, (j >> 5) + 1) << (32 - (j & 31));
+  }
+  const int left = k1 - key;
+  return left <= 0 ? 0u : left >= 32 ? v : v & ((1u << left) - 1);
+}
+
+template <int D, bool kQ>
+__global__ void __launch_bounds__(kThreads, 1)
+    tree_attention_tc_kernel(const __grid_constant__ Maps maps, const TreeAttention p, int mtiles, int max_splits,
+                             int num_pages) {
+  using C = Cfg<D, kQ>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* q_full = bars + 0;
+  uint64_t* k_full = bars + 1;    // [3]
+  uint64_t* k_empty = bars + 4;   // [3]
+  uint64_t* v_land = bars + 7;    // [2] TMA brought V (raw codes, or BF16)
+  uint64_t* v_full = bars + 9;    // [2] V as the MMA reads it
+  uint64_t* v_empty = bars + 11;  // [2]
+  uint64_t* r_empty = bars + 13;  // [2] raw codes converted
+  uint64_t* s_full = bars + 15;   // [2]
+  uint64_t* p_full = bars + 17;   // [2]
+  uint64_t* c_full = bars + 19;   // [4] the tile's scales are written
+  uint64_t* done = bars + 23;     // every MMA completed
+  uint64_t* joined = bars + 24;   // (B) the second warpgroup's sums are in shared memory
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* odd_v = reinterpret_cast<int*>(tmem_slot + 2);  // values that are not finite were left out
+  float* scales = reinterpret_cast<float*>(smem + C::kOffScale);
+  int* exps = reinterpret_cast<int*>(scales + kSlots * 2 * kTile);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = p.q_heads / p.kv_heads;
+  int item = blockIdx.x;
+  const int mt = item % mtiles;
+  item /= mtiles;
+  const int kvh = item % p.kv_heads;
+  const int split = blockIdx.y;
+  pdl_wait();
+  pdl_trigger();
+  const Segment seg = p.segments[item / p.kv_heads];
+  if (seg.len == 0) return;
+  if (!rows_fit(p, seg) || !segment_fits(p, seg)) {
+    if (mt == 0 && split == 0) {
+      if (threadIdx.x == 0) record_status(p.status, kBadArgument);
+      if (rows_fit(p, seg))
+        for (long i = threadIdx.x; i < (long)seg.len * G * D; i += kThreads)
+          p.o[(long)(seg.row_start + i / (G * D)) * p.ld_o + (long)kvh * G * D + i % (G * D)] = __float2bfloat16_rn(0.f);
+    }
+    return;
+  }
+  const int M = seg.len * G;
+  const int m0 = mt * 2 * kTile;
+  const int keys = seg.cached + seg.len;
+  const int nsplit = (keys + p.keys_per_split - 1) / p.keys_per_split;
+  if (m0 >= M || split >= nsplit) return;
+  const int k0 = split * p.keys_per_split;
+  const int k1 = min(keys, k0 + p.keys_per_split);
+  const int ntiles = (k1 - k0 + kTile - 1) / kTile;
+  const bool two = M - m0 > kTile;          // (A) two row tiles
+  const int steps = two ? 2 * ntiles : ntiles;  // (warpgroup, key tile) pairs in turn
+  const int32_t* table = p.table + seg.table_start;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, two ? 256 : 128);
+    for (int s = 0; s < 3; ++s) {
+      mbar_init(k_full + s, 1);
+      mbar_init(k_empty + s, 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(v_land + s, 1);
+      mbar_init(v_full + s, 128);
+      mbar_init(v_empty + s, 1);
+      mbar_init(r_empty + s, 128);
+      mbar_init(s_full + s, 1);
+      mbar_init(p_full + s, 128);
+    }
+    for (int s = 0; s < kSlots; ++s) mbar_init(c_full + s, 128);
+    mbar_init(done, 1);
+    mbar_init(joined, 128);
+    *abort = 0;
+    *odd_v = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&maps.cache);
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 9) {
+    // ------------------------------------------------------------------ loader
+    if (elect_one()) {
+      auto page_of = [&](int j, int pg, int which) -> int {  // page index of tile j's page, or past the last
+        const int b = k0 / 16 + j * 8 + pg;
+        if (j >= ntiles || b * 16 >= k1) return num_pages;
+        const int id = table[b];
+        if (id < 0 || id >= p.cache_blocks) {
+          record_status(p.status, kBadIndex);  // reads as zeros
+          return num_pages;
+        }
+        return (id * 2 + which) * p.kv_heads + kvh;
+      };
+      int kp[8], vp[8];
+      auto pages = [&](int j) {
+#pragma unroll
+        for (int pg = 0; pg < 8; ++pg) {
+          kp[pg] = page_of(j, pg, 0);
+          vp[pg] = kp[pg] == num_pages ? num_pages : kp[pg] + p.kv_heads;
+        }
+      };
+      auto load = [&](uint8_t* dst, uint64_t* bar, const int (&pages)[8]) {
+        mbar_arrive_expect_tx(bar, C::kKStage);
+#pragma unroll
+        for (int pg = 0; pg < 8; ++pg) {
+          if constexpr (kQ) {
+            tma_load_3d(dst + pg * 16 * D, &maps.cache, bar, 0, 0, pages[pg]);
+          } else {
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h)
+              tma_load_2d(dst + h * C::kHalf + pg * 2048, &maps.cache, bar, h * 64, pages[pg] * 16);
+          }
+        }
+      };
+      pages(0);
+      int got_k = 0, got_v = 0;
+      for (int j = 0; j < ntiles; ++j) {
+        const int ks = j % C::kKStages, vs = j & 1;
+        if (j >= C::kKStages && !mbar_wait(k_empty + ks, (j / C::kKStages + 1) & 1, p.status, kTimeoutSmemEmpty, abort)) break;
+        load(smem + C::kOffK + ks * C::kKStage, k_full + ks, kp);
+        ++got_k;
+        if (j >= 2 && !mbar_wait((kQ ? r_empty : v_empty) + vs, (j / 2 + 1) & 1, p.status, kTimeoutSmemEmpty, abort)) break;
+        load(smem + (kQ ? C::kOffRaw + vs * C::kTile8 : C::kOffV + vs * C::kTile16), v_land + vs, vp);
+        ++got_v;
+        pages(j + 1);
+      }
+      // Let the loads in flight land before the CTA may exit (an abort stops the loop early).
+      for (int j = got_k > C::kKStages ? got_k - C::kKStages : 0; j < got_k; ++j)
+        mbar_wait(k_full + j % C::kKStages, (j / C::kKStages) & 1, p.status, kTimeoutDrain, nullptr);
+      for (int j = got_v > 2 ? got_v - 2 : 0; j < got_v; ++j)
+        mbar_wait(v_land + (j & 1), (j / 2) & 1, p.status, kTimeoutDrain, nullptr);
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (elect_one()) {
+      constexpr uint32_t idesc_s = kQ ? idesc_e4m3_f32(kTile, kTile) : idesc_bf16_f32(kTile, kTile);
+      // P V: FP16 (format 0) over codes, BF16 else; B (V) MN-major.
+      constexpr uint32_t idesc_o = (kQ ? idesc_bf16_f32(kTile, D) & ~((1u << 7) | (1u << 10)) : idesc_bf16_f32(kTile, D)) | (1u << 16);
+      bool ok = mbar_wait(q_full, 0, p.status, kTimeoutTmemFull, abort);
+      auto scores = [&](int n) -> bool {
+        const int w = n & 1, j = two ? n >> 1 : n, ks = j % C::kKStages;
+        if (!mbar_wait(k_full + ks, (j / C::kKStages) & 1, p.status, kTimeoutTmaFull, abort)) return false;
+        tc_fence_after();
+        const uint8_t* kt = smem + C::kOffK + ks * C::kKStage;
+        const uint8_t* qt = smem + C::kOffQ + (two ? w : 0) * C::kQTile;
+        if constexpr (kQ) {
+#pragma unroll
+          for (int part = 0; part < 2; ++part)
+#pragma unroll
+            for (int kk = 0; kk < D / 32; ++kk)
+              mma_e4m3(tmem + w * kTile, desc_k8<D>(qt + part * C::kTile8 + kk * 32), desc_k8<D>(kt + kk * 32), idesc_s,
+                       part > 0 || kk > 0 ? 1u : 0u);
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            mma_bf16(tmem + w * kTile, sdesc_kmajor_sw128(qt + (kk >> 2) * C::kHalf + (kk & 3) * 32),
+                     sdesc_kmajor_sw128(kt + (kk >> 2) * C::kHalf + (kk & 3) * 32), idesc_s, kk > 0 ? 1u : 0u);
+        }
+        mma_commit(s_full + w);
+        if (!two || w == 1) mma_commit(k_empty + ks);
+        return true;
+      };
+      for (int n = 0; ok && n < 2 && n < steps; ++n) ok = scores(n);
+      for (int n = 0; ok && n < steps; ++n) {
+        const int w = n & 1, j = two ? n >> 1 : n, vs = j & 1;
+        if (!mbar_wait(p_full + w, (n >> 1) & 1, p.status, kTimeoutTmemFull, abort) ||
+            !mbar_wait(v_full + vs, (j / 2) & 1, p.status, kTimeoutTmaFull, abort))
+          break;
+        tc_fence_after();
+        const uint8_t* vt = smem + C::kOffV + vs * C::kTile16;
+#pragma unroll
+        for (int kk = 0; kk < kTile / 16; ++kk)
+          mma_f16_ts(tmem + C::kColO + w * kTile, tmem + w * kTile + kk * 8, desc_mn16(vt + kk * 2048, C::kHalf, 1024),
+                     idesc_o, n >= 2 || kk > 0 ? 1u : 0u);
+        if (!two || w == 1) mma_commit(v_empty + vs);
+        if (n + 2 < steps) ok = scores(n + 2);
+      }
+      // No MMA may still write TMEM when it is read or freed (an abort can leave some in flight).
+      mma_commit(done);
+      mbar_wait(done, 0, p.status, kTimeoutDrain, nullptr);
+    }
+  } else if (warp >= 10) {
+    // ------------------------------------------------------------------ helpers
+    const int i = threadIdx.x - 320;  // 0 .. 127: a key of the tile
+    const uint8_t* cache = static_cast<const uint8_t*>(p.cache);
+    float ks = 0.f, vs_ = 0.f;
+    auto fetch = [&](int j) {  // the scales of this thread's key of tile j
+      ks = vs_ = 0.f;
+      const int key = k0 + j * kTile + i;
+      if (j >= ntiles || key >= k1) return;
+      const int id = table[key >> 4];
+      if (id < 0 || id >= p.cache_blocks) return;
+      const long pb = 16L * D + kScaleBytes;
+      const uint8_t* at = cache + ((long)id * 2 * p.kv_heads + kvh) * pb + 16 * D + (key & 15) * 4;
+      ks = __ldg(reinterpret_cast<const float*>(at));
+      vs_ = __ldg(reinterpret_cast<const float*>(at + p.kv_heads * pb));
+    };
+    if constexpr (kQ) fetch(0);
+    bool odd = false;
+    for (int j = 0; j < ntiles; ++j) {
+      const int vs = j & 1, kb = k0 + j * kTile;
+      const bool inner = kb + kTile <= min(seg.cached, k1);
+      uint8_t* vt = smem + C::kOffV + vs * C::kTile16;
+      if constexpr (kQ) {
+        // The V stage's last reader (tile j - 2) is done, and with it the slot's (tile j - 4).
+        if (j >= 2 && !mbar_wait(v_empty + vs, (j / 2 + 1) & 1, p.status, kTimeoutTmemEmpty, abort)) break;
+        const int slot = j % kSlots;
+        float* sk = scales + slot * 2 * kTile;
+        const uint32_t mine = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs_, 0.f)));
+        sk[i] = ks;
+        sk[kTile + i] = vs_;
+        // Each warp's largest V scale, by its bits (scales are not negative).
+        if (lane == 0) exps[slot * 4 + (i >> 5)] = (int)mine;
+        mbar_arrive(c_full + slot);
+        fetch(j + 1);
+      }
+      if (!mbar_wait(v_land + vs, (j / 2) & 1, p.status, kTimeoutTmaFull, abort)) break;
+      if constexpr (kQ) {
+        const uint32_t raw = smem_u32(smem + C::kOffRaw + vs * C::kTile8);
+        const uint32_t dst = smem_u32(vt);
+        constexpr int kCh = D / 16;
+#pragma unroll
+        for (int u0 = 0; u0 < kCh; ++u0) {
+          const int u = i + u0 * 128, key = u / kCh, rc = u % kCh;
+          uint4 x = lds128(raw + at8<D>(key, rc));
+          uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          if (!inner && kb + key >= seg.cached) {
+            // A product with a zero weight must stay zero.
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (kb + key >= k1) w[e] = 0u;
+              for (int y = 0; y < 32; y += 8)
+                if ((w[e] >> y & 0x7fu) == 0x7fu) {
+                  w[e] &= ~(0xffu << y);
+                  odd = true;
+                }
+            }
+          }
+          const uint4 lo = make_uint4(e4m3x2_f16x2(w[0]), e4m3x2_f16x2_hi(w[0]), e4m3x2_f16x2(w[1]), e4m3x2_f16x2_hi(w[1]));
+          const uint4 hi = make_uint4(e4m3x2_f16x2(w[2]), e4m3x2_f16x2_hi(w[2]), e4m3x2_f16x2(w[3]), e4m3x2_f16x2_hi(w[3]));
+          // Lanes of the upper half of the columns store their chunks in the other order, so that
+          // a store's lanes fall in different banks.
+          const bool swap = kCh > 4 && rc >= 4;
+          sts128(dst + at16(key, 2 * rc + (swap ? 1 : 0)), swap ? hi : lo);
+          sts128(dst + at16(key, 2 * rc + (swap ? 0 : 1)), swap ? lo : hi);
+        }
+        mbar_arrive(r_empty + vs);
+      } else if (!inner) {
+        const uint32_t dst = smem_u32(vt);
+        constexpr int kCh = D / 8;
+        for (int u = i; u < kTile * kCh; u += 128) {
+          const int key = u / kCh;
+          if (kb + key < seg.cached) continue;
+          const uint32_t a = dst + at16(key, u % kCh);
+          uint4 x = lds128(a);
+          uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          bool change = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t bad = 0u;
+            if (kb + key >= k1) {
+              bad = ~0u;
+            } else {
+              if ((w[e] & 0x7f80u) == 0x7f80u) bad |= 0xffffu;
+              if ((w[e] & 0x7f800000u) == 0x7f800000u) bad |= 0xffff0000u;
+              if (bad != 0u) odd = true;
+            }
+            change = change || bad != 0u;
+            w[e] &= ~bad;
+          }
+          if (change) sts128(a, make_uint4(w[0], w[1], w[2], w[3]));
+        }
+      }
+      if (odd) atomicExch(odd_v, 1);
+      fence_proxy_async();
+      mbar_arrive(v_full + vs);
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax, a thread a row
+    const int w = warp >> 2;                          // warpgroup
+    const int row = threadIdx.x & 127;                // TMEM lane
+    const int m = m0 + (two ? w * kTile : 0) + row;
+    const bool real = m < M;
+    const int tok = real ? m / G : 0, head = kvh * G + (real ? m % G : 0);
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t s_col = lane_base + w * kTile, o_col = lane_base + C::kColO + w * kTile;
+    // Q: this row into the tile (by the first warpgroup alone where both share it).
+    float c = fmaxf(fabsf(p.scale) * kLog2e, 1.2e-38f);  // (a negative scale turns q's sign)
+    {
+      const __nv_bfloat16* src = p.q + (long)(seg.row_start + tok) * p.ld_q + (long)head * D;
+      const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
+      const uint32_t dst = smem_u32(smem + C::kOffQ + (two ? w : 0) * C::kQTile);
+      const bool store = two || w == 0;
+      if constexpr (kQ) {
+        float amax = 0.f;
+        if (real)
+#pragma unroll 4
+          for (int ch = 0; ch < D / 8; ++ch) {
+            const uint4 v = reinterpret_cast<const uint4*>(src)[ch];
+            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(bf16_lo(v.x)), fabsf(bf16_hi(v.x))), fmaxf(fabsf(bf16_lo(v.y)), fabsf(bf16_hi(v.y)))));
+            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(bf16_lo(v.z)), fabsf(bf16_hi(v.z))), fmaxf(fabsf(bf16_lo(v.w)), fabsf(bf16_hi(v.w)))));
+          }
+        const int e = min(max((int)(__float_as_uint(amax) >> 23), 8), 254) - 127;
+        const float down = __uint_as_float((uint32_t)(127 + 7 - e) << 23);  // 7 - e in [-120, 126]
+        c = fmaxf(c * __uint_as_float((uint32_t)(127 - 7 + e) << 23), 1.2e-38f);
+        if (store)
+#pragma unroll 2
+          for (int ch = 0; ch < D / 16; ++ch) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              uint4 v = make_uint4(0u, 0u, 0u, 0u);
+              if (real) v = reinterpret_cast<const uint4*>(src)[2 * ch + half];
+              const uint32_t vw[4] = {v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip};
+              uint16_t h[4], l[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                float2 f = make_float2(bf16_lo(vw[x]) * down, bf16_hi(vw[x]) * down);
+                if (!(fabsf(f.x) < INFINITY)) f.x = __int_as_float(0x7fffffff);  // (the conversion saturates)
+                if (!(fabsf(f.y) < INFINITY)) f.y = __int_as_float(0x7fffffff);
+                h[x] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+                const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2(h[x], __NV_E4M3);
+                const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&hr));
+                l[x] = __nv_cvt_float2_to_fp8x2(make_float2(f.x - hf.x, f.y - hf.y), __NV_SATFINITE, __NV_E4M3);
+              }
+              hi[2 * half] = h[0] | (uint32_t)h[1] << 16;
+              hi[2 * half + 1] = h[2] | (uint32_t)h[3] << 16;
+              lo[2 * half] = l[0] | (uint32_t)l[1] << 16;
+              lo[2 * half + 1] = l[2] | (uint32_t)l[3] << 16;
+            }
+            sts128(dst + at8<D>(row, ch), make_uint4(hi[0], hi[1], hi[2], hi[3]));
+            sts128(dst + C::kTile8 + at8<D>(row, ch), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+          }
+      } else if (store) {
+#pragma unroll 4
+        for (int ch = 0; ch < D / 8; ++ch) {
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (real) v = reinterpret_cast<const uint4*>(src)[ch];
+          sts128(dst + at16(row, ch), make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip));
+        }
+      }
+      if (store) {
+        fence_proxy_async();
+        mbar_arrive(q_full);
+      }
+    }
+    const bool idle = !__any_sync(0xffffffffu, real);  // none of the warp's rows counts
+    float top = -INFINITY, sum = 0.f;
+    int v_exp = -126;
+    bool ok = true;
+    int i = 0;
+    for (int n = w; n < steps; n += 2, ++i) {
+      const int j = two ? i : n, kb = k0 + j * kTile;
+      int got = 1;
+      if (lane == 0) got = mbar_wait(s_full + w, i & 1, p.status, kTimeoutTmemFull, abort);
+      if (!__shfl_sync(0xffffffffu, got, 0)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int slot = j % kSlots;
+      if constexpr (kQ) {
+        const bool there = mbar_wait(c_full + slot, (j / kSlots) & 1, p.status, kTimeoutTmemFull, abort);
+        if (!__all_sync(0xffffffffu, there)) {
+          ok = false;
+          break;
+        }
+      }
+      if (!idle) {
+        const float* sk = scales + slot * 2 * kTile;
+        const bool inner = kb + kTile <= min(seg.cached, k1);
+        // The row's largest score of the tile (over K's scales; c is positive).
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c0 = 0; c0 < kTile; c0 += 32) {
+          uint32_t r[32];
+          __syncwarp();
+          tmem_ld_32x32b_x32(s_col + c0, r);
+          tmem_ld_wait();
+          const uint32_t seen = inner ? ~0u : visible(p, seg, tok, kb + c0, k1);
+#pragma unroll
+          for (int x = 0; x < 32; x += 4) {
+            float4 k4 = make_float4(1.f, 1.f, 1.f, 1.f);
+            if constexpr (kQ) k4 = *reinterpret_cast<const float4*>(sk + c0 + x);
+            float2 a = make_float2(__uint_as_float(r[x]), __uint_as_float(r[x + 1]));
+            float2 b = make_float2(__uint_as_float(r[x + 2]), __uint_as_float(r[x + 3]));
+            if constexpr (kQ) {
+              a = mul2(a, make_float2(k4.x, k4.y));
+              b = mul2(b, make_float2(k4.z, k4.w));
+            }
+            if (!inner) {
+              a.x = seen >> x & 1u ? a.x : -INFINITY;
+              a.y = seen >> (x + 1) & 1u ? a.y : -INFINITY;
+              b.x = seen >> (x + 2) & 1u ? b.x : -INFINITY;
+              b.y = seen >> (x + 3) & 1u ? b.y : -INFINITY;
+            }
+            mx = fmaxf(mx, fmaxf(fmaxf(a.x, a.y), fmaxf(b.x, b.y)));
+          }
+        }
+        if (mx > -INFINITY) mx *= c;
+        float f = 1.f, fo = 1.f;
+        if (mx > top + kSlack) {
+          f = top == -INFINITY ? 0.f : ex2(top - mx);
+          fo = f;
+          top = mx;
+        }
+        float v_inv = 1.f;
+        if constexpr (kQ) {
+          const int4 warps = *reinterpret_cast<const int4*>(exps + slot * 4);
+          const int e = min(max(max(max(warps.x, warps.y), max(warps.z, warps.w)) >> 23, 1), 253) - 127;
+          if (e > v_exp) {
+            fo *= ex2((float)(v_exp - e));
+            v_exp = e;
+          }
+          v_inv = __uint_as_float((uint32_t)(127 - v_exp) << 23);
+        }
+        sum *= f;
+        // (S_w of this step follows P_w V of the one before: O may be changed.)
+        if (i > 0 && __any_sync(0xffffffffu, fo != 1.f)) {
+#pragma unroll
+          for (int c0 = 0; c0 < D; c0 += 32) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(o_col + c0, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int x = 0; x < 32; ++x) r[x] = __float_as_uint(__uint_as_float(r[x]) * fo);
+            tmem_st_32x32b_x32(o_col + c0, r);
+          }
+        }
+        // Weights: P takes the columns of scores that were read already.
+        const float z = top == -INFINITY ? 0.f : top - kLift;
+        const float2 c2 = make_float2(c, c), z2 = make_float2(-z, -z), v2 = make_float2(v_inv, v_inv);
+        float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int c0 = 0; c0 < kTile; c0 += 32) {
+          uint32_t r[32], out[16];
+          __syncwarp();
+          tmem_ld_32x32b_x32(s_col + c0, r);
+          tmem_ld_wait();
+          const uint32_t seen = inner ? ~0u : visible(p, seg, tok, kb + c0, k1);
+#pragma unroll
+          for (int x = 0; x < 32; x += 4) {
+            float2 a = make_float2(__uint_as_float(r[x]), __uint_as_float(r[x + 1]));
+            float2 b = make_float2(__uint_as_float(r[x + 2]), __uint_as_float(r[x + 3]));
+            if constexpr (kQ) {
+              const float4 k4 = *reinterpret_cast<const float4*>(sk + c0 + x);
+              a = mul2(a, make_float2(k4.x, k4.y));
+              b = mul2(b, make_float2(k4.z, k4.w));
+            }
+            a = fma2(a, c2, z2);
+            b = fma2(b, c2, z2);
+            if (!inner) {
+              a.x = seen >> x & 1u ? a.x : -INFINITY;
+              a.y = seen >> (x + 1) & 1u ? a.y : -INFINITY;
+              b.x = seen >> (x + 2) & 1u ? b.x : -INFINITY;
+              b.y = seen >> (x + 3) & 1u ? b.y : -INFINITY;
+            }
+            a = make_float2(ex2(a.x), ex2(a.y));
+            b = make_float2(ex2(b.x), ex2(b.y));
+            acc = add2(acc, add2(a, b));
+            if constexpr (kQ) {
+              const float4 v4 = *reinterpret_cast<const float4*>(sk + kTile + c0 + x);
+              a = mul2(a, mul2(make_float2(v4.x, v4.y), v2));
+              b = mul2(b, mul2(make_float2(v4.z, v4.w), v2));
+              out[x / 2] = pack_f16x2(a.x, a.y);
+              out[x / 2 + 1] = pack_f16x2(b.x, b.y);
+            } else {
+              out[x / 2] = pack_bf16x2(a.x, a.y);
+              out[x / 2 + 1] = pack_bf16x2(b.x, b.y);
+            }
+          }
+          __syncwarp();
+          tmem_st_32x32b_x16(s_col + c0 / 2, out);
+        }
+        sum += acc.x + acc.y;
+        tmem_st_wait();
+      }
+      tc_fence_before();
+      mbar_arrive(p_full + w);
+    }
+    // Every MMA done, O holds the sums (none for a warpgroup without a step).
+    int fine = ok ? 1 : 0;
+    if (ok && lane == 0) fine = mbar_wait(done, 0, p.status, kTimeoutTmemFull, abort);
+    fine = __shfl_sync(0xffffffffu, fine, 0);
+    tc_fence_after();
+    const float back = kQ ? __uint_as_float((uint32_t)(127 + v_exp) << 23) : 1.f;
+    float* row_top = reinterpret_cast<float*>(smem + C::kOffRow);
+    float* row_sum = row_top + kTile;
+    // (B) The second warpgroup's sums go through the key and value stages, free by now.
+    float* other = reinterpret_cast<float*>(smem + C::kOffK);
+    static_assert(kTile * D * 4 <= C::kOffScale - C::kOffK, "the join fits the stages");
+    auto other_at = [&](int ch) { return other + row * D + ((ch ^ row) & (D / 4 - 1)) * 4; };  // 4 columns
+    if (!two && w == 1) {
+      if (fine) {
+        row_top[row] = i > 0 ? top : -INFINITY;
+        row_sum[row] = sum;
+        if (i > 0 && !idle) {
+#pragma unroll
+          for (int c0 = 0; c0 < D; c0 += 32) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(o_col + c0, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int x = 0; x < 32; x += 4)
+              *reinterpret_cast<float4*>(other_at((c0 + x) / 4)) =
+                  make_float4(__uint_as_float(r[x]) * back, __uint_as_float(r[x + 1]) * back,
+                              __uint_as_float(r[x + 2]) * back, __uint_as_float(r[x + 3]) * back);
+          }
+        }
+      }
+      mbar_arrive(joined);
+    } else {
+      if (!two && fine) fine = mbar_wait(joined, 0, p.status, kTimeoutTmemFull, abort);
+      fine = __all_sync(0xffffffffu, fine);
+      if (fine && !idle) {
+        float f0 = 1.f, f1 = 0.f;
+        if (!two) {
+          const float t1 = row_top[row], both = fmaxf(top, t1);
+          f0 = top == -INFINITY ? 0.f : ex2(top - both);
+          f1 = t1 == -INFINITY ? 0.f : ex2(t1 - both);
+          sum = sum * f0 + row_sum[row] * f1;
+          top = both;
+        }
+        const bool fix = *reinterpret_cast<volatile int*>(odd_v) != 0;
+        const float norm = nsplit > 1 ? 1.f : top == -INFINITY ? 0.f : 1.f / sum;
+        const long at = (long)(seg.row_start + tok);
+        const long idx = (at * p.q_heads + head) * max_splits + split;
+        __nv_bfloat16* dst = p.o + at * p.ld_o + (long)head * D;
+        float* part = p.partial_o + idx * D;
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t r[32];
+          __syncwarp();
+          tmem_ld_32x32b_x32(o_col + c0, r);
+          tmem_ld_wait();
+          float v[32];
+#pragma unroll
+          for (int x = 0; x < 32; ++x) v[x] = __uint_as_float(r[x]) * back * f0;
+          if (f1 > 0.f) {
+#pragma unroll
+            for (int x = 0; x < 32; x += 4) {
+              const float4 y = *reinterpret_cast<const float4*>(other_at((c0 + x) / 4));
+              v[x] = fmaf(y.x, f1, v[x]);
+              v[x + 1] = fmaf(y.y, f1, v[x + 1]);
+              v[x + 2] = fmaf(y.z, f1, v[x + 2]);
+              v[x + 3] = fmaf(y.w, f1, v[x + 3]);
+            }
+          }
+          if (real && fix) {
+            const uint8_t* cache = static_cast<const uint8_t*>(p.cache);
+            const long pb = kQ ? 16L * D + kScaleBytes : 32L * D;
+            for (int a = max(0, k0 - seg.cached); a < min(seg.len, k1 - seg.cached); ++a) {
+              if (!(mask_word(p, seg, tok, a >> 5) >> (a & 31) & 1u)) continue;
+              const int key = seg.cached + a, id = table[key >> 4];
+              if (id < 0 || id >= p.cache_blocks) continue;
+              const uint8_t* vp = cache + ((long)id * 2 * p.kv_heads + p.kv_heads + kvh) * pb + (long)(key & 15) * D * (kQ ? 1 : 2);
+#pragma unroll
+              for (int x = 0; x < 32; ++x) {
+                if constexpr (kQ) {
+                  if ((vp[c0 + x] & 0x7fu) == 0x7fu) v[x] = __int_as_float(0x7fffffff);
+                } else {
+                  const float y = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(vp)[c0 + x]);
+                  if (!(fabsf(y) < INFINITY)) v[x] += y;
+                }
+              }
+            }
+          }
+          if (real && nsplit == 1) {
+#pragma unroll
+            for (int x = 0; x < 32; x += 8)
+              *reinterpret_cast<uint4*>(dst + c0 + x) =
+                  make_uint4(pack_bf16x2(v[x] * norm, v[x + 1] * norm), pack_bf16x2(v[x + 2] * norm, v[x + 3] * norm),
+                             pack_bf16x2(v[x + 4] * norm, v[x + 5] * norm), pack_bf16x2(v[x + 6] * norm, v[x + 7] * norm));
+          } else if (real) {
+#pragma unroll
+            for (int x = 0; x < 32; x += 4)
+              *reinterpret_cast<float4*>(part + c0 + x) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+          }
+        }
+        if (real && nsplit > 1) p.partial_ml[idx] = make_float2(top, sum);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Codes: [pages][16 rows][D] bytes, a page's rows together and its scales behind them.
+bool encode_codes(CUtensorMap* map, const void* base, long pages, int d) {
+  auto fn = tmap_encoder();
+  if (fn == nullptr) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)d, 16, (cuuint64_t)pages};
+  cuuint64_t strides[2] = {(cuuint64_t)d, (cuuint64_t)quantized_page_bytes(d)};
+  cuuint32_t box[3] = {(cuuint32_t)d, 16, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool kQ>
+int launch(const TreeAttention& p, int splits, cudaStream_t stream) {
+  using C = Cfg<D, kQ>;
+  static_assert(C::kSmem <= 232448, "shared memory");
+  const int G = p.q_heads / p.kv_heads;
+  const long mtiles = ((long)p.max_len * G + 2 * kTile - 1) / (2 * kTile);
+  const long ctas = mtiles * p.kv_heads * p.num_segments;
+  if (ctas > 2147483647L) return -2;
+  const long pages = p.cache_blocks * 2 * p.kv_heads;
+  Maps maps;
+  if (kQ ? !encode_codes(&maps.cache, p.cache, pages, D)
+         : !encode_tmap_2d(&maps.cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.cache, pages * 16, D, D, 16, 64,
+                           CU_TENSOR_MAP_SWIZZLE_128B))
+    return -4;
+  const auto kernel = tree_attention_tc_kernel<D, kQ>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess) return -5;
+  return launch_pdl(kernel, dim3((unsigned)ctas, splits), dim3(kThreads), C::kSmem, stream, maps, p, (int)mtiles, splits,
+                    (int)pages) == cudaSuccess
+             ? 0
+             : -5;
+}
+
+}  // namespace
+
+bool tree_attention_tc_supported(const TreeAttention& p) {
+  const long pages = p.cache_blocks * 2 * p.kv_heads;
+  return p.cache_blocks > 0 && pages * 16 < (1L << 31) - 16 && (p.head_dim == 64 || p.head_dim == 128);
+}
+
+int tree_attention_tc(const TreeAttention& p, cudaStream_t stream) {
+  if (!tree_attention_tc_supported(p)) return -2;
+  const int splits = (p.max_keys + p.keys_per_split - 1) / p.keys_per_split;
+  if (p.head_dim == 64) return p.quantized ? launch<64, true>(p, splits, stream) : launch<64, false>(p, splits, stream);
+  return p.quantized ? launch<128, true>(p, splits, stream) : launch<128, false>(p, splits, stream);
+}
+
+}  // namespace foa

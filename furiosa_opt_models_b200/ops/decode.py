@@ -238,8 +238,8 @@ def paged_tree(q, cache, table, segments, kv_heads, max_keys, max_len, mask=None
         if splits > 1:
             need = rows * q_heads * splits
             work = torch.empty(need * (d + 2), dtype=torch.float32, device=q.device)
-            pl = work.data_ptr()
-            po = pl + need * 8
+            po = work.data_ptr()
+            pl = po + need * d * 4
         ops.tree_attention(
             q.data_ptr(), q.stride(0) if rows > 1 else q_heads * d, out.data_ptr(),
             out.stride(0) if rows > 1 else q_heads * d, rows, pages.data_ptr(), quantized, pages.shape[0],

@@ -200,7 +200,7 @@ def _attend64(q, values, table, segs, scale, mask=None, causal=True):
     """(outputs, tolerances) of the formula in 64 bits. ``mask``: per segment, bool [len, len]."""
     rows, hq, d = q.shape
     hk = values.shape[2]
-    out, weight, err = (torch.zeros(rows, hq, d, dtype=F64) for _ in range(3))
+    out, weight, err, part = (torch.zeros(rows, hq, d, dtype=F64) for _ in range(4))
     for i, (row, n, c, start, nb) in enumerate(segs):
         if n == 0:
             continue
@@ -217,16 +217,23 @@ def _attend64(q, values, table, segs, scale, mask=None, causal=True):
             p_v = torch.where(p[..., None] > 0, p[..., None] * seen, 0.0)
             out[row:row + n, h] = p_v.sum(1)
             weight[row:row + n, h] = p_v.abs().sum(1)
-            err[row:row + n, h] = ((qh.abs() @ kh.abs().nan_to_num(0.0).T) * scale).masked_fill(~see, 0).amax(-1, keepdim=True)
-    return out, weight, err
+            mags = kh.abs().nan_to_num(0.0)
+            err[row:row + n, h] = ((qh.abs() @ mags.T) * scale).masked_fill(~see, 0).amax(-1, keepdim=True)
+            most = qh.abs().amax(-1, keepdim=True) * mags.sum(-1) * scale
+            part[row:row + n, h] = most.masked_fill(~see, 0).amax(-1, keepdim=True)
+    return out, weight, (err, part)
 
 
 def _tolerance(ref, weight, err, d, quantized):
     """One rounding of the output, one of each weight (FP16 over codes, BF16 over BF16), and the
     scores' FP32 sums of d products (and two scalings), each off by 2^-24 of the sum of magnitudes;
-    a weight and its sum feel that twice. ex2 and lg2 add 2^-21 each."""
+    a weight and its sum feel that twice. ex2 and lg2 add 2^-21 each. Over codes q may enter as two
+    E4M3 parts of a row scaled to [128, 256): BF16's 8 bits are two parts of 4, so only bits below
+    E4M3's smallest step 2^-9 are rounded, by 2^-10 at most, which is 2^-17 of the row's largest."""
+    err, part = err
     return _half(BF16) * ref.abs() + weight * (
-        _half(torch.float16 if quantized else BF16) + 2 * (d + 4) * 2.0 ** -24 * err + 2.0 ** -20)
+        _half(torch.float16 if quantized else BF16) + 2 * (d + 4) * 2.0 ** -24 * err + 2.0 ** -20
+        + (2 * 2.0 ** -17 * part if quantized else 0))
 
 
 def _random_masks(lens, gen, empty=False):
@@ -690,7 +697,7 @@ def test_a_speculative_step():
                                  step.d ** -0.5, mask=ms)
     # q rounds to BF16 in the kernel from FP32 and here from FP64: a step apart at most, which moves
     # each score by 2^-8 of its sum of magnitudes at worst.
-    tol = _tolerance(ref, weight, err, step.d, True) + 2 * _half(BF16) * 2 * weight * err
+    tol = _tolerance(ref, weight, err, step.d, True) + 2 * _half(BF16) * 2 * weight * err[0]
     assert ((o.double().cpu() - ref).abs() <= tol).all()
     lists = drafted["output"][0].view(11, 6).tolist()
     bits = (drafted["allowed"].cpu().long()[:, :, None] >> torch.arange(32)).flatten(1) & 1 == 1
