@@ -16,8 +16,9 @@
 //   E4M3 would lose a long tail of small probabilities; they write the keys' scales beside it.
 // - BF16 pages: TMA brings K and V as the MMAs read them; the helpers only clear V rows past the
 //   keys and values that are not finite.
-// - Row maxima move when a tile exceeds them by 2^4, V's reference scale when a tile's largest
-//   does (tracked by the helpers): O is rescaled in TMEM then.
+// - Row maxima move when a tile exceeds them by 2^4, the reference exponent of V's scales when a
+//   tile's largest does; O is rescaled in TMEM then. Both are part of the unit that O and the row's
+//   sum are held in.
 // - Every wait is bounded; a timeout records a status and every role leaves through the same end.
 //
 // Over quantized pages with 256 rows the MMAs bound it (two FP8 passes of S cost what one FP16 pass
@@ -25,6 +26,8 @@
 
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
+
+#include <type_traits>
 
 #include "decode_ops.cuh"
 #include "launch.cuh"
@@ -37,8 +40,9 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLift = 10.f;   // weights are scaled by 2^10 ...
 constexpr float kSlack = 4.f;   // ... and may exceed the row's reference maximum by 2^4
+constexpr int kLeastExp = -90;  // least exponent of V's reference scale (sums stay below 2^127)
 constexpr int kTile = 128;      // rows and keys of an MMA tile
-constexpr int kThreads = 448;   // 8 softmax warps, MMA, loader, 4 helpers
+constexpr int kThreads = 448;   // 8 softmax warps, MMA, loader, 4 helpers (128 registers a thread)
 constexpr int kSlots = 4;       // key tiles whose scales are held
 
 template <int D, bool kQ>
@@ -120,12 +124,11 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32"
-      " [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
+// tcgen05.wait::ld whose loaded values cannot be used before it.
+__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
 
 // Shared-memory descriptors: a K-major 8-bit operand in rows of `kRowBytes` (128 or 64, swizzled over
@@ -156,6 +159,16 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
       " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+
+// mbar_wait by one lane for its warp: polls of whole warps fill the queue that shared-memory loads
+// go through (a softmax step took 7,500 cycles instead of 3,000 beside four polling warps).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status, int site, volatile int* abort) {
+  int got = 1;
+  if ((threadIdx.x & 31) == 0) got = mbar_wait(bar, parity, status, site, abort);
+  got = __shfl_sync(0xffffffffu, got, 0);
+  __syncwarp();
+  return got != 0;
 }
 
 // 16-byte chunk `c` of row `r` in rows of kRowBytes as TMA swizzles them.
@@ -291,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 9) {
     // ------------------------------------------------------------------ loader
     if (elect_one()) {
-      auto page_of = [&](int j, int pg, int which) -> int {  // page index of tile j's page, or past the last
+      auto page_of = [&](int j, int pg) -> int {  // K's page index of tile j's page, or one past the last
         const int b = k0 / 16 + j * 8 + pg;
         if (j >= ntiles || b * 16 >= k1) return num_pages;
         const int id = table[b];
@@ -299,26 +312,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           record_status(p.status, kBadIndex);  // reads as zeros
           return num_pages;
         }
-        return (id * 2 + which) * p.kv_heads + kvh;
+        return id * 2 * p.kv_heads + kvh;
       };
-      int kp[8], vp[8];
+      int kp[8];  // read a tile ahead
       auto pages = [&](int j) {
 #pragma unroll
-        for (int pg = 0; pg < 8; ++pg) {
-          kp[pg] = page_of(j, pg, 0);
-          vp[pg] = kp[pg] == num_pages ? num_pages : kp[pg] + p.kv_heads;
-        }
+        for (int pg = 0; pg < 8; ++pg) kp[pg] = page_of(j, pg);
       };
-      auto load = [&](uint8_t* dst, uint64_t* bar, const int (&pages)[8]) {
+      auto load = [&](uint8_t* dst, uint64_t* bar, int up) {  // the pages `up` heads further
         mbar_arrive_expect_tx(bar, C::kKStage);
 #pragma unroll
         for (int pg = 0; pg < 8; ++pg) {
+          const int page = kp[pg] == num_pages ? num_pages : kp[pg] + up;
           if constexpr (kQ) {
-            tma_load_3d(dst + pg * 16 * D, &maps.cache, bar, 0, 0, pages[pg]);
+            tma_load_3d(dst + pg * 16 * D, &maps.cache, bar, 0, 0, page);
           } else {
 #pragma unroll
             for (int h = 0; h < D / 64; ++h)
-              tma_load_2d(dst + h * C::kHalf + pg * 2048, &maps.cache, bar, h * 64, pages[pg] * 16);
+              tma_load_2d(dst + h * C::kHalf + pg * 2048, &maps.cache, bar, h * 64, page * 16);
           }
         }
       };
@@ -327,10 +338,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; j < ntiles; ++j) {
         const int ks = j % C::kKStages, vs = j & 1;
         if (j >= C::kKStages && !mbar_wait(k_empty + ks, (j / C::kKStages + 1) & 1, p.status, kTimeoutSmemEmpty, abort)) break;
-        load(smem + C::kOffK + ks * C::kKStage, k_full + ks, kp);
+        load(smem + C::kOffK + ks * C::kKStage, k_full + ks, 0);
         ++got_k;
         if (j >= 2 && !mbar_wait((kQ ? r_empty : v_empty) + vs, (j / 2 + 1) & 1, p.status, kTimeoutSmemEmpty, abort)) break;
-        load(smem + (kQ ? C::kOffRaw + vs * C::kTile8 : C::kOffV + vs * C::kTile16), v_land + vs, vp);
+        load(smem + (kQ ? C::kOffRaw + vs * C::kTile8 : C::kOffV + vs * C::kTile16), v_land + vs, p.kv_heads);
         ++got_v;
         pages(j + 1);
       }
@@ -413,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint8_t* vt = smem + C::kOffV + vs * C::kTile16;
       if constexpr (kQ) {
         // The V stage's last reader (tile j - 2) is done, and with it the slot's (tile j - 4).
-        if (j >= 2 && !mbar_wait(v_empty + vs, (j / 2 + 1) & 1, p.status, kTimeoutTmemEmpty, abort)) break;
+        if (j >= 2 && !warp_wait(v_empty + vs, (j / 2 + 1) & 1, p.status, kTimeoutTmemEmpty, abort)) break;
         const int slot = j % kSlots;
         float* sk = scales + slot * 2 * kTile;
         const uint32_t mine = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs_, 0.f)));
@@ -424,12 +435,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(c_full + slot);
         fetch(j + 1);
       }
-      if (!mbar_wait(v_land + vs, (j / 2) & 1, p.status, kTimeoutTmaFull, abort)) break;
+      if (!warp_wait(v_land + vs, (j / 2) & 1, p.status, kTimeoutTmaFull, abort)) break;
       if constexpr (kQ) {
         const uint32_t raw = smem_u32(smem + C::kOffRaw + vs * C::kTile8);
         const uint32_t dst = smem_u32(vt);
         constexpr int kCh = D / 16;
-#pragma unroll
+#pragma unroll 2
         for (int u0 = 0; u0 < kCh; ++u0) {
           const int u = i + u0 * 128, key = u / kCh, rc = u % kCh;
           uint4 x = lds128(raw + at8<D>(key, rc));
@@ -556,22 +567,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     const bool idle = !__any_sync(0xffffffffu, real);  // none of the warp's rows counts
     float top = -INFINITY, sum = 0.f;
-    int v_exp = -126;
+    int v_exp = kQ ? kLeastExp : 0;  // O and the sums are in units of 2^(top + v_exp - 10)
     bool ok = true;
     int i = 0;
     for (int n = w; n < steps; n += 2, ++i) {
       const int j = two ? i : n, kb = k0 + j * kTile;
-      int got = 1;
-      if (lane == 0) got = mbar_wait(s_full + w, i & 1, p.status, kTimeoutTmemFull, abort);
-      if (!__shfl_sync(0xffffffffu, got, 0)) {
+      if (!warp_wait(s_full + w, i & 1, p.status, kTimeoutTmemFull, abort)) {
         ok = false;
         break;
       }
       tc_fence_after();
       const int slot = j % kSlots;
       if constexpr (kQ) {
-        const bool there = mbar_wait(c_full + slot, (j / kSlots) & 1, p.status, kTimeoutTmemFull, abort);
-        if (!__all_sync(0xffffffffu, there)) {
+        if (!warp_wait(c_full + slot, (j / kSlots) & 1, p.status, kTimeoutTmemFull, abort)) {
           ok = false;
           break;
         }
@@ -579,77 +587,86 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!idle) {
         const float* sk = scales + slot * 2 * kTile;
         const bool inner = kb + kTile <= min(seg.cached, k1);
-        // The row's largest score of the tile (over K's scales; c is positive).
-        float mx = -INFINITY;
+        int e = v_exp;
+        if constexpr (kQ) {
+          const int4 warps = *reinterpret_cast<const int4*>(exps + slot * 4);
+          e = max(v_exp, min(max(max(warps.x, warps.y), max(warps.z, warps.w)) >> 23, 253) - 127);
+        }
+        const float2 c2 = make_float2(c, c);
+        // Two passes over S, 16 columns at a time with the next ones on their way: the row's largest
+        // score (over K's scales; c is positive), then the weights by the reference moved to it.
+        // Loops are kept rolled: their code is shared by eight warps beside four other roles.
+        float mx0 = -INFINITY, mx1 = -INFINITY;
+        uint32_t ra[16], rb[16];
+        auto largest = [&](const uint32_t (&r)[16], int c0, auto masked, uint32_t seen) {
 #pragma unroll
-        for (int c0 = 0; c0 < kTile; c0 += 32) {
-          uint32_t r[32];
-          __syncwarp();
-          tmem_ld_32x32b_x32(s_col + c0, r);
-          tmem_ld_wait();
-          const uint32_t seen = inner ? ~0u : visible(p, seg, tok, kb + c0, k1);
-#pragma unroll
-          for (int x = 0; x < 32; x += 4) {
-            float4 k4 = make_float4(1.f, 1.f, 1.f, 1.f);
-            if constexpr (kQ) k4 = *reinterpret_cast<const float4*>(sk + c0 + x);
+          for (int x = 0; x < 16; x += 4) {
             float2 a = make_float2(__uint_as_float(r[x]), __uint_as_float(r[x + 1]));
             float2 b = make_float2(__uint_as_float(r[x + 2]), __uint_as_float(r[x + 3]));
             if constexpr (kQ) {
+              const float4 k4 = *reinterpret_cast<const float4*>(sk + c0 + x);
               a = mul2(a, make_float2(k4.x, k4.y));
               b = mul2(b, make_float2(k4.z, k4.w));
             }
-            if (!inner) {
+            if constexpr (decltype(masked)::value) {
               a.x = seen >> x & 1u ? a.x : -INFINITY;
               a.y = seen >> (x + 1) & 1u ? a.y : -INFINITY;
               b.x = seen >> (x + 2) & 1u ? b.x : -INFINITY;
               b.y = seen >> (x + 3) & 1u ? b.y : -INFINITY;
             }
-            mx = fmaxf(mx, fmaxf(fmaxf(a.x, a.y), fmaxf(b.x, b.y)));
+            mx0 = fmaxf(mx0, fmaxf(a.x, a.y));
+            mx1 = fmaxf(mx1, fmaxf(b.x, b.y));
           }
-        }
+        };
+        auto first_pass = [&](auto masked) {
+          tmem_ld_32x32b_x16(s_col, ra);
+#pragma unroll 1
+          for (int c0 = 0; c0 < kTile; c0 += 32) {
+            uint32_t seen = ~0u;
+            if constexpr (decltype(masked)::value) {
+              seen = visible(p, seg, tok, kb + c0, k1);
+              __syncwarp();
+            }
+            tmem_wait16(ra);
+            tmem_ld_32x32b_x16(s_col + c0 + 16, rb);
+            largest(ra, c0, masked, seen);
+            tmem_wait16(rb);
+            if (c0 + 32 < kTile) tmem_ld_32x32b_x16(s_col + c0 + 32, ra);
+            largest(rb, c0 + 16, masked, seen >> 16);
+          }
+        };
+        if (inner)
+          first_pass(std::false_type{});
+        else
+          first_pass(std::true_type{});
+        float mx = fmaxf(mx0, mx1), f = 1.f;
         if (mx > -INFINITY) mx *= c;
-        float f = 1.f, fo = 1.f;
         if (mx > top + kSlack) {
           f = top == -INFINITY ? 0.f : ex2(top - mx);
-          fo = f;
           top = mx;
         }
-        float v_inv = 1.f;
-        if constexpr (kQ) {
-          const int4 warps = *reinterpret_cast<const int4*>(exps + slot * 4);
-          const int e = min(max(max(max(warps.x, warps.y), max(warps.z, warps.w)) >> 23, 1), 253) - 127;
-          if (e > v_exp) {
-            fo *= ex2((float)(v_exp - e));
-            v_exp = e;
-          }
-          v_inv = __uint_as_float((uint32_t)(127 - v_exp) << 23);
+        if (e != v_exp) {
+          f *= ex2((float)(v_exp - e));
+          v_exp = e;
         }
         sum *= f;
         // (S_w of this step follows P_w V of the one before: O may be changed.)
-        if (i > 0 && __any_sync(0xffffffffu, fo != 1.f)) {
+        if (i > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < D; c0 += 16) {
+            tmem_ld_32x32b_x16(o_col + c0, ra);
+            tmem_wait16(ra);
 #pragma unroll
-          for (int c0 = 0; c0 < D; c0 += 32) {
-            uint32_t r[32];
-            tmem_ld_32x32b_x32(o_col + c0, r);
-            tmem_ld_wait();
-#pragma unroll
-            for (int x = 0; x < 32; ++x) r[x] = __float_as_uint(__uint_as_float(r[x]) * fo);
-            tmem_st_32x32b_x32(o_col + c0, r);
+            for (int x = 0; x < 16; ++x) ra[x] = __float_as_uint(__uint_as_float(ra[x]) * f);
+            tmem_st_32x32b_x16(o_col + c0, ra);
           }
         }
-        // Weights: P takes the columns of scores that were read already.
-        const float z = top == -INFINITY ? 0.f : top - kLift;
-        const float2 c2 = make_float2(c, c), z2 = make_float2(-z, -z), v2 = make_float2(v_inv, v_inv);
-        float2 acc = make_float2(0.f, 0.f);
+        const float z = top == -INFINITY ? 0.f : top + (float)v_exp - kLift;
+        const float2 z2 = make_float2(-z, -z);
+        float2 acc0 = make_float2(0.f, 0.f), acc1 = acc0;
+        auto weights = [&](const uint32_t (&r)[16], int c0, auto masked, uint32_t seen, uint32_t* out) {
 #pragma unroll
-        for (int c0 = 0; c0 < kTile; c0 += 32) {
-          uint32_t r[32], out[16];
-          __syncwarp();
-          tmem_ld_32x32b_x32(s_col + c0, r);
-          tmem_ld_wait();
-          const uint32_t seen = inner ? ~0u : visible(p, seg, tok, kb + c0, k1);
-#pragma unroll
-          for (int x = 0; x < 32; x += 4) {
+          for (int x = 0; x < 16; x += 4) {
             float2 a = make_float2(__uint_as_float(r[x]), __uint_as_float(r[x + 1]));
             float2 b = make_float2(__uint_as_float(r[x + 2]), __uint_as_float(r[x + 3]));
             if constexpr (kQ) {
@@ -659,7 +676,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             a = fma2(a, c2, z2);
             b = fma2(b, c2, z2);
-            if (!inner) {
+            if constexpr (decltype(masked)::value) {
               a.x = seen >> x & 1u ? a.x : -INFINITY;
               a.y = seen >> (x + 1) & 1u ? a.y : -INFINITY;
               b.x = seen >> (x + 2) & 1u ? b.x : -INFINITY;
@@ -667,11 +684,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             a = make_float2(ex2(a.x), ex2(a.y));
             b = make_float2(ex2(b.x), ex2(b.y));
-            acc = add2(acc, add2(a, b));
+            acc0 = add2(acc0, a);
+            acc1 = add2(acc1, b);
             if constexpr (kQ) {
               const float4 v4 = *reinterpret_cast<const float4*>(sk + kTile + c0 + x);
-              a = mul2(a, mul2(make_float2(v4.x, v4.y), v2));
-              b = mul2(b, mul2(make_float2(v4.z, v4.w), v2));
+              a = mul2(a, make_float2(v4.x, v4.y));
+              b = mul2(b, make_float2(v4.z, v4.w));
               out[x / 2] = pack_f16x2(a.x, a.y);
               out[x / 2 + 1] = pack_f16x2(b.x, b.y);
             } else {
@@ -679,21 +697,41 @@ __global__ void __launch_bounds__(kThreads, 1)
               out[x / 2 + 1] = pack_bf16x2(b.x, b.y);
             }
           }
-          __syncwarp();
-          tmem_st_32x32b_x16(s_col + c0 / 2, out);
-        }
-        sum += acc.x + acc.y;
+        };
+        // P takes the columns of scores that were read already.
+        auto second_pass = [&](auto masked) {
+          tmem_ld_32x32b_x16(s_col, ra);
+#pragma unroll 1
+          for (int c0 = 0; c0 < kTile; c0 += 32) {
+            uint32_t seen = ~0u;
+            if constexpr (decltype(masked)::value) {
+              seen = visible(p, seg, tok, kb + c0, k1);
+              __syncwarp();
+            }
+            uint32_t out[16];
+            tmem_wait16(ra);
+            tmem_ld_32x32b_x16(s_col + c0 + 16, rb);
+            weights(ra, c0, masked, seen, out);
+            tmem_wait16(rb);
+            if (c0 + 32 < kTile) tmem_ld_32x32b_x16(s_col + c0 + 32, ra);
+            weights(rb, c0 + 16, masked, seen >> 16, out + 8);
+            tmem_st_32x32b_x16(s_col + c0 / 2, out);
+          }
+        };
+        if (inner)
+          second_pass(std::false_type{});
+        else
+          second_pass(std::true_type{});
+        sum += (acc0.x + acc0.y) + (acc1.x + acc1.y);
         tmem_st_wait();
       }
       tc_fence_before();
       mbar_arrive(p_full + w);
     }
     // Every MMA done, O holds the sums (none for a warpgroup without a step).
-    int fine = ok ? 1 : 0;
-    if (ok && lane == 0) fine = mbar_wait(done, 0, p.status, kTimeoutTmemFull, abort);
-    fine = __shfl_sync(0xffffffffu, fine, 0);
+    bool fine = ok && warp_wait(done, 0, p.status, kTimeoutTmemFull, abort);
     tc_fence_after();
-    const float back = kQ ? __uint_as_float((uint32_t)(127 + v_exp) << 23) : 1.f;
+    top += (float)v_exp;
     float* row_top = reinterpret_cast<float*>(smem + C::kOffRow);
     float* row_sum = row_top + kTile;
     // (B) The second warpgroup's sums go through the key and value stages, free by now.
@@ -713,15 +751,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int x = 0; x < 32; x += 4)
               *reinterpret_cast<float4*>(other_at((c0 + x) / 4)) =
-                  make_float4(__uint_as_float(r[x]) * back, __uint_as_float(r[x + 1]) * back,
-                              __uint_as_float(r[x + 2]) * back, __uint_as_float(r[x + 3]) * back);
+                  make_float4(__uint_as_float(r[x]), __uint_as_float(r[x + 1]), __uint_as_float(r[x + 2]),
+                              __uint_as_float(r[x + 3]));
           }
         }
       }
       mbar_arrive(joined);
     } else {
-      if (!two && fine) fine = mbar_wait(joined, 0, p.status, kTimeoutTmemFull, abort);
-      fine = __all_sync(0xffffffffu, fine);
+      if (!two && fine) fine = warp_wait(joined, 0, p.status, kTimeoutTmemFull, abort);
       if (fine && !idle) {
         float f0 = 1.f, f1 = 0.f;
         if (!two) {
@@ -737,7 +774,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const long idx = (at * p.q_heads + head) * max_splits + split;
         __nv_bfloat16* dst = p.o + at * p.ld_o + (long)head * D;
         float* part = p.partial_o + idx * D;
-#pragma unroll
+#pragma unroll 1
         for (int c0 = 0; c0 < D; c0 += 32) {
           uint32_t r[32];
           __syncwarp();
@@ -745,7 +782,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld_wait();
           float v[32];
 #pragma unroll
-          for (int x = 0; x < 32; ++x) v[x] = __uint_as_float(r[x]) * back * f0;
+          for (int x = 0; x < 32; ++x) v[x] = __uint_as_float(r[x]) * f0;
           if (f1 > 0.f) {
 #pragma unroll
             for (int x = 0; x < 32; x += 4) {
