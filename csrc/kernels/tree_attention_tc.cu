@@ -27,8 +27,6 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
-#include <type_traits>
-
 #include "decode_ops.cuh"
 #include "launch.cuh"
 #include "sm100.cuh"
@@ -42,7 +40,10 @@ constexpr float kLift = 10.f;   // weights are scaled by 2^10 ...
 constexpr float kSlack = 4.f;   // ... and may exceed the row's reference maximum by 2^4
 constexpr int kLeastExp = -90;  // least exponent of V's reference scale (sums stay below 2^127)
 constexpr int kTile = 128;      // rows and keys of an MMA tile
-constexpr int kThreads = 448;   // 8 softmax warps, MMA, loader, 4 helpers (128 registers a thread)
+constexpr int kThreads = 512;   // 8 softmax warps, MMA, loader, 4 helpers, 2 idle (whole warpgroups)
+// Registers a thread: 128 at the launch (512 x 128 is the SM's file), moved between warpgroups.
+constexpr int kSoftmaxRegs = 192, kOtherRegs = 64;
+static_assert(256 * kSoftmaxRegs + 256 * kOtherRegs == kThreads * 128, "the shares are the launch's registers");
 constexpr int kSlots = 4;       // key tiles whose scales are held
 
 template <int D, bool kQ>
@@ -161,14 +162,31 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
       : "memory");
 }
 
-// mbar_wait by one lane for its warp: polls of whole warps fill the queue that shared-memory loads
-// go through (a softmax step took 7,500 cycles instead of 3,000 beside four polling warps).
+// Bounded waits of one thread and of a whole warp, in few instructions (sm100's with its clock, at
+// twenty places beside five roles' code, pushed the softmax loop out of the instruction cache). A
+// poll blocks for some time by itself; the limit is on their number.
+constexpr uint32_t kPolls = 1u << 22;
+__device__ __forceinline__ bool gave_up(uint32_t polls, int* status, int site, volatile int* abort) {
+  if (polls & 63u) return false;
+  if (abort != nullptr && *abort) return true;
+  if (polls < kPolls) return false;
+  record_status(status, site);
+  if (abort != nullptr) *abort = 1;
+  return true;
+}
+__device__ __forceinline__ bool wait1(uint64_t* bar, uint32_t parity, int* status, int site, volatile int* abort) {
+  const uint32_t at = smem_u32(bar);
+  uint32_t polls = 0;
+  while (!mbar_try_wait(at, parity))
+    if (gave_up(++polls, status, site, abort)) return false;
+  return true;
+}
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status, int site, volatile int* abort) {
-  int got = 1;
-  if ((threadIdx.x & 31) == 0) got = mbar_wait(bar, parity, status, site, abort);
-  got = __shfl_sync(0xffffffffu, got, 0);
-  __syncwarp();
-  return got != 0;
+  const uint32_t at = smem_u32(bar);
+  uint32_t polls = 0;
+  while (!__all_sync(0xffffffffu, mbar_try_wait(at, parity)))
+    if (__any_sync(0xffffffffu, gave_up(++polls, status, site, abort))) return false;
+  return true;
 }
 
 // 16-byte chunk `c` of row `r` in rows of kRowBytes as TMA swizzles them.
@@ -253,8 +271,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (mt == 0 && split == 0) {
       if (threadIdx.x == 0) record_status(p.status, kBadArgument);
       if (rows_fit(p, seg))
-        for (long i = threadIdx.x; i < (long)seg.len * G * D; i += kThreads)
-          p.o[(long)(seg.row_start + i / (G * D)) * p.ld_o + (long)kvh * G * D + i % (G * D)] = __float2bfloat16_rn(0.f);
+        for (int r = 0; r < seg.len; ++r)
+          for (int x = threadIdx.x; x < G * D; x += kThreads)
+            p.o[(long)(seg.row_start + r) * p.ld_o + (long)kvh * G * D + x] = __float2bfloat16_rn(0.f);
     }
     return;
   }
@@ -301,202 +320,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 9) {
-    // ------------------------------------------------------------------ loader
-    if (elect_one()) {
-      auto page_of = [&](int j, int pg) -> int {  // K's page index of tile j's page, or one past the last
-        const int b = k0 / 16 + j * 8 + pg;
-        if (j >= ntiles || b * 16 >= k1) return num_pages;
-        const int id = table[b];
-        if (id < 0 || id >= p.cache_blocks) {
-          record_status(p.status, kBadIndex);  // reads as zeros
-          return num_pages;
-        }
-        return id * 2 * p.kv_heads + kvh;
-      };
-      int kp[8];  // read a tile ahead
-      auto pages = [&](int j) {
-#pragma unroll
-        for (int pg = 0; pg < 8; ++pg) kp[pg] = page_of(j, pg);
-      };
-      auto load = [&](uint8_t* dst, uint64_t* bar, int up) {  // the pages `up` heads further
-        mbar_arrive_expect_tx(bar, C::kKStage);
-#pragma unroll
-        for (int pg = 0; pg < 8; ++pg) {
-          const int page = kp[pg] == num_pages ? num_pages : kp[pg] + up;
-          if constexpr (kQ) {
-            tma_load_3d(dst + pg * 16 * D, &maps.cache, bar, 0, 0, page);
-          } else {
-#pragma unroll
-            for (int h = 0; h < D / 64; ++h)
-              tma_load_2d(dst + h * C::kHalf + pg * 2048, &maps.cache, bar, h * 64, page * 16);
-          }
-        }
-      };
-      pages(0);
-      int got_k = 0, got_v = 0;
-      for (int j = 0; j < ntiles; ++j) {
-        const int ks = j % C::kKStages, vs = j & 1;
-        if (j >= C::kKStages && !mbar_wait(k_empty + ks, (j / C::kKStages + 1) & 1, p.status, kTimeoutSmemEmpty, abort)) break;
-        load(smem + C::kOffK + ks * C::kKStage, k_full + ks, 0);
-        ++got_k;
-        if (j >= 2 && !mbar_wait((kQ ? r_empty : v_empty) + vs, (j / 2 + 1) & 1, p.status, kTimeoutSmemEmpty, abort)) break;
-        load(smem + (kQ ? C::kOffRaw + vs * C::kTile8 : C::kOffV + vs * C::kTile16), v_land + vs, p.kv_heads);
-        ++got_v;
-        pages(j + 1);
-      }
-      // Let the loads in flight land before the CTA may exit (an abort stops the loop early).
-      for (int j = got_k > C::kKStages ? got_k - C::kKStages : 0; j < got_k; ++j)
-        mbar_wait(k_full + j % C::kKStages, (j / C::kKStages) & 1, p.status, kTimeoutDrain, nullptr);
-      for (int j = got_v > 2 ? got_v - 2 : 0; j < got_v; ++j)
-        mbar_wait(v_land + (j & 1), (j / 2) & 1, p.status, kTimeoutDrain, nullptr);
-    }
-  } else if (warp == 8) {
-    // ------------------------------------------------------------------ MMA issuer
-    if (elect_one()) {
-      constexpr uint32_t idesc_s = kQ ? idesc_e4m3_f32(kTile, kTile) : idesc_bf16_f32(kTile, kTile);
-      // P V: FP16 (format 0) over codes, BF16 else; B (V) MN-major.
-      constexpr uint32_t idesc_o = (kQ ? idesc_bf16_f32(kTile, D) & ~((1u << 7) | (1u << 10)) : idesc_bf16_f32(kTile, D)) | (1u << 16);
-      bool ok = mbar_wait(q_full, 0, p.status, kTimeoutTmemFull, abort);
-      auto scores = [&](int n) -> bool {
-        const int w = n & 1, j = two ? n >> 1 : n, ks = j % C::kKStages;
-        if (!mbar_wait(k_full + ks, (j / C::kKStages) & 1, p.status, kTimeoutTmaFull, abort)) return false;
-        tc_fence_after();
-        const uint8_t* kt = smem + C::kOffK + ks * C::kKStage;
-        const uint8_t* qt = smem + C::kOffQ + (two ? w : 0) * C::kQTile;
-        if constexpr (kQ) {
-#pragma unroll
-          for (int part = 0; part < 2; ++part)
-#pragma unroll
-            for (int kk = 0; kk < D / 32; ++kk)
-              mma_e4m3(tmem + w * kTile, desc_k8<D>(qt + part * C::kTile8 + kk * 32), desc_k8<D>(kt + kk * 32), idesc_s,
-                       part > 0 || kk > 0 ? 1u : 0u);
-        } else {
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            mma_bf16(tmem + w * kTile, sdesc_kmajor_sw128(qt + (kk >> 2) * C::kHalf + (kk & 3) * 32),
-                     sdesc_kmajor_sw128(kt + (kk >> 2) * C::kHalf + (kk & 3) * 32), idesc_s, kk > 0 ? 1u : 0u);
-        }
-        mma_commit(s_full + w);
-        if (!two || w == 1) mma_commit(k_empty + ks);
-        return true;
-      };
-      for (int n = 0; ok && n < 2 && n < steps; ++n) ok = scores(n);
-      for (int n = 0; ok && n < steps; ++n) {
-        const int w = n & 1, j = two ? n >> 1 : n, vs = j & 1;
-        if (!mbar_wait(p_full + w, (n >> 1) & 1, p.status, kTimeoutTmemFull, abort) ||
-            !mbar_wait(v_full + vs, (j / 2) & 1, p.status, kTimeoutTmaFull, abort))
-          break;
-        tc_fence_after();
-        const uint8_t* vt = smem + C::kOffV + vs * C::kTile16;
-#pragma unroll
-        for (int kk = 0; kk < kTile / 16; ++kk)
-          mma_f16_ts(tmem + C::kColO + w * kTile, tmem + w * kTile + kk * 8, desc_mn16(vt + kk * 2048, C::kHalf, 1024),
-                     idesc_o, n >= 2 || kk > 0 ? 1u : 0u);
-        if (!two || w == 1) mma_commit(v_empty + vs);
-        if (n + 2 < steps) ok = scores(n + 2);
-      }
-      // No MMA may still write TMEM when it is read or freed (an abort can leave some in flight).
-      mma_commit(done);
-      mbar_wait(done, 0, p.status, kTimeoutDrain, nullptr);
-    }
-  } else if (warp >= 10) {
-    // ------------------------------------------------------------------ helpers
-    const int i = threadIdx.x - 320;  // 0 .. 127: a key of the tile
-    const uint8_t* cache = static_cast<const uint8_t*>(p.cache);
-    float ks = 0.f, vs_ = 0.f;
-    auto fetch = [&](int j) {  // the scales of this thread's key of tile j
-      ks = vs_ = 0.f;
-      const int key = k0 + j * kTile + i;
-      if (j >= ntiles || key >= k1) return;
-      const int id = table[key >> 4];
-      if (id < 0 || id >= p.cache_blocks) return;
-      const long pb = 16L * D + kScaleBytes;
-      const uint8_t* at = cache + ((long)id * 2 * p.kv_heads + kvh) * pb + 16 * D + (key & 15) * 4;
-      ks = __ldg(reinterpret_cast<const float*>(at));
-      vs_ = __ldg(reinterpret_cast<const float*>(at + p.kv_heads * pb));
-    };
-    if constexpr (kQ) fetch(0);
-    bool odd = false;
-    for (int j = 0; j < ntiles; ++j) {
-      const int vs = j & 1, kb = k0 + j * kTile;
-      const bool inner = kb + kTile <= min(seg.cached, k1);
-      uint8_t* vt = smem + C::kOffV + vs * C::kTile16;
-      if constexpr (kQ) {
-        // The V stage's last reader (tile j - 2) is done, and with it the slot's (tile j - 4).
-        if (j >= 2 && !warp_wait(v_empty + vs, (j / 2 + 1) & 1, p.status, kTimeoutTmemEmpty, abort)) break;
-        const int slot = j % kSlots;
-        float* sk = scales + slot * 2 * kTile;
-        const uint32_t mine = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs_, 0.f)));
-        sk[i] = ks;
-        sk[kTile + i] = vs_;
-        // Each warp's largest V scale, by its bits (scales are not negative).
-        if (lane == 0) exps[slot * 4 + (i >> 5)] = (int)mine;
-        mbar_arrive(c_full + slot);
-        fetch(j + 1);
-      }
-      if (!warp_wait(v_land + vs, (j / 2) & 1, p.status, kTimeoutTmaFull, abort)) break;
-      if constexpr (kQ) {
-        const uint32_t raw = smem_u32(smem + C::kOffRaw + vs * C::kTile8);
-        const uint32_t dst = smem_u32(vt);
-        constexpr int kCh = D / 16;
-#pragma unroll 2
-        for (int u0 = 0; u0 < kCh; ++u0) {
-          const int u = i + u0 * 128, key = u / kCh, rc = u % kCh;
-          uint4 x = lds128(raw + at8<D>(key, rc));
-          uint32_t w[4] = {x.x, x.y, x.z, x.w};
-          if (!inner && kb + key >= seg.cached) {
-            // A product with a zero weight must stay zero.
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (kb + key >= k1) w[e] = 0u;
-              for (int y = 0; y < 32; y += 8)
-                if ((w[e] >> y & 0x7fu) == 0x7fu) {
-                  w[e] &= ~(0xffu << y);
-                  odd = true;
-                }
-            }
-          }
-          const uint4 lo = make_uint4(e4m3x2_f16x2(w[0]), e4m3x2_f16x2_hi(w[0]), e4m3x2_f16x2(w[1]), e4m3x2_f16x2_hi(w[1]));
-          const uint4 hi = make_uint4(e4m3x2_f16x2(w[2]), e4m3x2_f16x2_hi(w[2]), e4m3x2_f16x2(w[3]), e4m3x2_f16x2_hi(w[3]));
-          // Lanes of the upper half of the columns store their chunks in the other order, so that
-          // a store's lanes fall in different banks.
-          const bool swap = kCh > 4 && rc >= 4;
-          sts128(dst + at16(key, 2 * rc + (swap ? 1 : 0)), swap ? hi : lo);
-          sts128(dst + at16(key, 2 * rc + (swap ? 0 : 1)), swap ? lo : hi);
-        }
-        mbar_arrive(r_empty + vs);
-      } else if (!inner) {
-        const uint32_t dst = smem_u32(vt);
-        constexpr int kCh = D / 8;
-        for (int u = i; u < kTile * kCh; u += 128) {
-          const int key = u / kCh;
-          if (kb + key < seg.cached) continue;
-          const uint32_t a = dst + at16(key, u % kCh);
-          uint4 x = lds128(a);
-          uint32_t w[4] = {x.x, x.y, x.z, x.w};
-          bool change = false;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t bad = 0u;
-            if (kb + key >= k1) {
-              bad = ~0u;
-            } else {
-              if ((w[e] & 0x7f80u) == 0x7f80u) bad |= 0xffffu;
-              if ((w[e] & 0x7f800000u) == 0x7f800000u) bad |= 0xffff0000u;
-              if (bad != 0u) odd = true;
-            }
-            change = change || bad != 0u;
-            w[e] &= ~bad;
-          }
-          if (change) sts128(a, make_uint4(w[0], w[1], w[2], w[3]));
-        }
-      }
-      if (odd) atomicExch(odd_v, 1);
-      fence_proxy_async();
-      mbar_arrive(v_full + vs);
-    }
-  } else {
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ------------------------------------------------------------------ softmax, a thread a row
     const int w = warp >> 2;                          // warpgroup
     const int row = threadIdx.x & 127;                // TMEM lane
@@ -592,53 +417,47 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int4 warps = *reinterpret_cast<const int4*>(exps + slot * 4);
           e = max(v_exp, min(max(max(warps.x, warps.y), max(warps.z, warps.w)) >> 23, 253) - 127);
         }
-        const float2 c2 = make_float2(c, c);
-        // Two passes over S, 16 columns at a time with the next ones on their way: the row's largest
-        // score (over K's scales; c is positive), then the weights by the reference moved to it.
-        // Loops are kept rolled: their code is shared by eight warps beside four other roles.
+        // The row's 128 scores stay in registers: K's scales, the mask and the largest as they arrive
+        // (c is positive, so the largest needs no scaling), then the weights.
+        uint32_t r[kTile];
         float mx0 = -INFINITY, mx1 = -INFINITY;
-        uint32_t ra[16], rb[16];
-        auto largest = [&](const uint32_t (&r)[16], int c0, auto masked, uint32_t seen) {
+        tmem_ld_32x32b_x32(s_col, *reinterpret_cast<uint32_t(*)[32]>(r));
 #pragma unroll
-          for (int x = 0; x < 16; x += 4) {
+        for (int c0 = 0; c0 < kTile; c0 += 32) {
+          tmem_wait16(*reinterpret_cast<uint32_t(*)[16]>(r + c0));
+          tmem_wait16(*reinterpret_cast<uint32_t(*)[16]>(r + c0 + 16));
+          if (c0 + 32 < kTile) tmem_ld_32x32b_x32(s_col + c0 + 32, *reinterpret_cast<uint32_t(*)[32]>(r + (c0 + 32) % kTile));
+#pragma unroll
+          for (int x = c0; x < c0 + 32; x += 4) {
             float2 a = make_float2(__uint_as_float(r[x]), __uint_as_float(r[x + 1]));
             float2 b = make_float2(__uint_as_float(r[x + 2]), __uint_as_float(r[x + 3]));
             if constexpr (kQ) {
-              const float4 k4 = *reinterpret_cast<const float4*>(sk + c0 + x);
+              const float4 k4 = *reinterpret_cast<const float4*>(sk + x);
               a = mul2(a, make_float2(k4.x, k4.y));
               b = mul2(b, make_float2(k4.z, k4.w));
-            }
-            if constexpr (decltype(masked)::value) {
-              a.x = seen >> x & 1u ? a.x : -INFINITY;
-              a.y = seen >> (x + 1) & 1u ? a.y : -INFINITY;
-              b.x = seen >> (x + 2) & 1u ? b.x : -INFINITY;
-              b.y = seen >> (x + 3) & 1u ? b.y : -INFINITY;
+              r[x] = __float_as_uint(a.x);
+              r[x + 1] = __float_as_uint(a.y);
+              r[x + 2] = __float_as_uint(b.x);
+              r[x + 3] = __float_as_uint(b.y);
             }
             mx0 = fmaxf(mx0, fmaxf(a.x, a.y));
             mx1 = fmaxf(mx1, fmaxf(b.x, b.y));
           }
-        };
-        auto first_pass = [&](auto masked) {
-          tmem_ld_32x32b_x16(s_col, ra);
-#pragma unroll 1
+        }
+        if (!inner) {
+          mx0 = mx1 = -INFINITY;
+#pragma unroll
           for (int c0 = 0; c0 < kTile; c0 += 32) {
-            uint32_t seen = ~0u;
-            if constexpr (decltype(masked)::value) {
-              seen = visible(p, seg, tok, kb + c0, k1);
-              __syncwarp();
+            const uint32_t seen = visible(p, seg, tok, kb + c0, k1);
+#pragma unroll
+            for (int x = 0; x < 32; ++x) {
+              const float t = seen >> x & 1u ? __uint_as_float(r[c0 + x]) : -INFINITY;
+              r[c0 + x] = __float_as_uint(t);
+              mx0 = fmaxf(mx0, t);
             }
-            tmem_wait16(ra);
-            tmem_ld_32x32b_x16(s_col + c0 + 16, rb);
-            largest(ra, c0, masked, seen);
-            tmem_wait16(rb);
-            if (c0 + 32 < kTile) tmem_ld_32x32b_x16(s_col + c0 + 32, ra);
-            largest(rb, c0 + 16, masked, seen >> 16);
           }
-        };
-        if (inner)
-          first_pass(std::false_type{});
-        else
-          first_pass(std::true_type{});
+          __syncwarp();
+        }
         float mx = fmaxf(mx0, mx1), f = 1.f;
         if (mx > -INFINITY) mx *= c;
         if (mx > top + kSlack) {
@@ -654,34 +473,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (i > 0 && __any_sync(0xffffffffu, f != 1.f)) {
 #pragma unroll 1
           for (int c0 = 0; c0 < D; c0 += 16) {
-            tmem_ld_32x32b_x16(o_col + c0, ra);
-            tmem_wait16(ra);
+            uint32_t y[16];
+            tmem_ld_32x32b_x16(o_col + c0, y);
+            tmem_wait16(y);
 #pragma unroll
-            for (int x = 0; x < 16; ++x) ra[x] = __float_as_uint(__uint_as_float(ra[x]) * f);
-            tmem_st_32x32b_x16(o_col + c0, ra);
+            for (int x = 0; x < 16; ++x) y[x] = __float_as_uint(__uint_as_float(y[x]) * f);
+            tmem_st_32x32b_x16(o_col + c0, y);
           }
         }
         const float z = top == -INFINITY ? 0.f : top + (float)v_exp - kLift;
-        const float2 z2 = make_float2(-z, -z);
+        const float2 c2 = make_float2(c, c), z2 = make_float2(-z, -z);
         float2 acc0 = make_float2(0.f, 0.f), acc1 = acc0;
-        auto weights = [&](const uint32_t (&r)[16], int c0, auto masked, uint32_t seen, uint32_t* out) {
+        // P takes the columns of S.
 #pragma unroll
-          for (int x = 0; x < 16; x += 4) {
-            float2 a = make_float2(__uint_as_float(r[x]), __uint_as_float(r[x + 1]));
-            float2 b = make_float2(__uint_as_float(r[x + 2]), __uint_as_float(r[x + 3]));
-            if constexpr (kQ) {
-              const float4 k4 = *reinterpret_cast<const float4*>(sk + c0 + x);
-              a = mul2(a, make_float2(k4.x, k4.y));
-              b = mul2(b, make_float2(k4.z, k4.w));
-            }
-            a = fma2(a, c2, z2);
-            b = fma2(b, c2, z2);
-            if constexpr (decltype(masked)::value) {
-              a.x = seen >> x & 1u ? a.x : -INFINITY;
-              a.y = seen >> (x + 1) & 1u ? a.y : -INFINITY;
-              b.x = seen >> (x + 2) & 1u ? b.x : -INFINITY;
-              b.y = seen >> (x + 3) & 1u ? b.y : -INFINITY;
-            }
+        for (int c0 = 0; c0 < kTile; c0 += 32) {
+          uint32_t out[16];
+#pragma unroll
+          for (int x = 0; x < 32; x += 4) {
+            float2 a = fma2(make_float2(__uint_as_float(r[c0 + x]), __uint_as_float(r[c0 + x + 1])), c2, z2);
+            float2 b = fma2(make_float2(__uint_as_float(r[c0 + x + 2]), __uint_as_float(r[c0 + x + 3])), c2, z2);
             a = make_float2(ex2(a.x), ex2(a.y));
             b = make_float2(ex2(b.x), ex2(b.y));
             acc0 = add2(acc0, a);
@@ -697,31 +507,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               out[x / 2 + 1] = pack_bf16x2(b.x, b.y);
             }
           }
-        };
-        // P takes the columns of scores that were read already.
-        auto second_pass = [&](auto masked) {
-          tmem_ld_32x32b_x16(s_col, ra);
-#pragma unroll 1
-          for (int c0 = 0; c0 < kTile; c0 += 32) {
-            uint32_t seen = ~0u;
-            if constexpr (decltype(masked)::value) {
-              seen = visible(p, seg, tok, kb + c0, k1);
-              __syncwarp();
-            }
-            uint32_t out[16];
-            tmem_wait16(ra);
-            tmem_ld_32x32b_x16(s_col + c0 + 16, rb);
-            weights(ra, c0, masked, seen, out);
-            tmem_wait16(rb);
-            if (c0 + 32 < kTile) tmem_ld_32x32b_x16(s_col + c0 + 32, ra);
-            weights(rb, c0 + 16, masked, seen >> 16, out + 8);
-            tmem_st_32x32b_x16(s_col + c0 / 2, out);
-          }
-        };
-        if (inner)
-          second_pass(std::false_type{});
-        else
-          second_pass(std::true_type{});
+          tmem_st_32x32b_x16(s_col + c0 / 2, out);
+        }
         sum += (acc0.x + acc0.y) + (acc1.x + acc1.y);
         tmem_st_wait();
       }
@@ -825,6 +612,215 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (real && nsplit > 1) p.partial_ml[idx] = make_float2(top, sum);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 9) {
+      // ------------------------------------------------------------------ loader, a lane a page
+      auto page_of = [&](int j) -> int {  // K's page index of this lane's page of tile j, or one past the last
+        const int b = k0 / 16 + j * 8 + lane;
+        if (j >= ntiles || lane >= 8 || b * 16 >= k1) return num_pages;
+        const int id = table[b];
+        if (id < 0 || id >= p.cache_blocks) {
+          record_status(p.status, kBadIndex);  // reads as zeros
+          return num_pages;
+        }
+        return id * 2 * p.kv_heads + kvh;
+      };
+      auto load = [&](uint8_t* dst, uint64_t* bar, int page) {
+        if (lane == 0) mbar_arrive_expect_tx(bar, C::kKStage);
+        __syncwarp();
+        if (lane < 8) {
+          if constexpr (kQ) {
+            tma_load_3d(dst + lane * 16 * D, &maps.cache, bar, 0, 0, page);
+          } else {
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h)
+              tma_load_2d(dst + h * C::kHalf + lane * 2048, &maps.cache, bar, h * 64, page * 16);
+          }
+        }
+        __syncwarp();
+      };
+      int got_k = 0, got_v = 0, next = page_of(0);
+      for (int j = 0; j < ntiles; ++j) {
+        const int ks = j % C::kKStages, vs = j & 1, page = next;
+        if (j >= C::kKStages && !warp_wait(k_empty + ks, (j / C::kKStages + 1) & 1, p.status, kTimeoutSmemEmpty, abort)) break;
+        load(smem + C::kOffK + ks * C::kKStage, k_full + ks, page);
+        ++got_k;
+        next = page_of(j + 1);
+        if (j >= 2 && !warp_wait((kQ ? r_empty : v_empty) + vs, (j / 2 + 1) & 1, p.status, kTimeoutSmemEmpty, abort)) break;
+        load(smem + (kQ ? C::kOffRaw + vs * C::kTile8 : C::kOffV + vs * C::kTile16), v_land + vs,
+             page == num_pages ? num_pages : page + p.kv_heads);
+        ++got_v;
+      }
+      // Let the loads in flight land before the CTA may exit (an abort stops the loop early).
+      for (int j = got_k > C::kKStages ? got_k - C::kKStages : 0; j < got_k; ++j)
+        warp_wait(k_full + j % C::kKStages, (j / C::kKStages) & 1, p.status, kTimeoutDrain, nullptr);
+      for (int j = got_v > 2 ? got_v - 2 : 0; j < got_v; ++j)
+        warp_wait(v_land + (j & 1), (j / 2) & 1, p.status, kTimeoutDrain, nullptr);
+    } else if (warp == 8) {
+      // ------------------------------------------------------------------ MMA issuer
+      if (elect_one()) {
+        constexpr uint32_t idesc_s = kQ ? idesc_e4m3_f32(kTile, kTile) : idesc_bf16_f32(kTile, kTile);
+        // P V: FP16 (format 0) over codes, BF16 else; B (V) MN-major.
+        constexpr uint32_t idesc_o = (kQ ? idesc_bf16_f32(kTile, D) & ~((1u << 7) | (1u << 10)) : idesc_bf16_f32(kTile, D)) | (1u << 16);
+        bool ok = wait1(q_full, 0, p.status, kTimeoutTmemFull, abort);
+        auto scores = [&](int n) -> bool {
+          const int w = n & 1, j = two ? n >> 1 : n, ks = j % C::kKStages;
+          if (!wait1(k_full + ks, (j / C::kKStages) & 1, p.status, kTimeoutTmaFull, abort)) return false;
+          tc_fence_after();
+          // (Descriptors of a tile's steps differ in their address field alone.)
+          const uint8_t* kt = smem + C::kOffK + ks * C::kKStage;
+          const uint8_t* qt = smem + C::kOffQ + (two ? w : 0) * C::kQTile;
+          const uint64_t kd = kQ ? desc_k8<D>(kt) : sdesc_kmajor_sw128(kt);
+          const uint64_t qd = kQ ? desc_k8<D>(qt) : sdesc_kmajor_sw128(qt);
+          if constexpr (kQ) {
+#pragma unroll
+            for (int part = 0; part < 2; ++part)
+#pragma unroll
+              for (int kk = 0; kk < D / 32; ++kk)
+                mma_e4m3(tmem + w * kTile, qd + ((part * C::kTile8 + kk * 32) >> 4), kd + (kk * 32 >> 4), idesc_s,
+                         part > 0 || kk > 0 ? 1u : 0u);
+          } else {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const int step = ((kk >> 2) * C::kHalf + (kk & 3) * 32) >> 4;
+              mma_bf16(tmem + w * kTile, qd + step, kd + step, idesc_s, kk > 0 ? 1u : 0u);
+            }
+          }
+          mma_commit(s_full + w);
+          if (!two || w == 1) mma_commit(k_empty + ks);
+          return true;
+        };
+        for (int n = -2; ok && n < steps; ++n) {
+          if (n >= 0) {
+            const int w = n & 1, j = two ? n >> 1 : n, vs = j & 1;
+            if (!wait1(p_full + w, (n >> 1) & 1, p.status, kTimeoutTmemFull, abort) ||
+                !wait1(v_full + vs, (j / 2) & 1, p.status, kTimeoutTmaFull, abort))
+              break;
+            tc_fence_after();
+            const uint64_t vd = desc_mn16(smem + C::kOffV + vs * C::kTile16, C::kHalf, 1024);
+#pragma unroll
+            for (int kk = 0; kk < kTile / 16; ++kk)
+              mma_f16_ts(tmem + C::kColO + w * kTile, tmem + w * kTile + kk * 8, vd + (kk * 2048 >> 4), idesc_o,
+                         n >= 2 || kk > 0 ? 1u : 0u);
+            if (!two || w == 1) mma_commit(v_empty + vs);
+          }
+          if (n + 2 < steps) ok = scores(n + 2);
+        }
+        // No MMA may still write TMEM when it is read or freed (an abort can leave some in flight).
+        mma_commit(done);
+        wait1(done, 0, p.status, kTimeoutDrain, nullptr);
+      }
+    } else if (warp < 14) {
+      // ------------------------------------------------------------------ helpers
+      const int i = threadIdx.x - 320;  // 0 .. 127: a key of the tile
+      const uint8_t* cache = static_cast<const uint8_t*>(p.cache);
+      float ks = 0.f, vs_ = 0.f;
+      auto fetch = [&](int j) {  // the scales of this thread's key of tile j
+        ks = vs_ = 0.f;
+        const int key = k0 + j * kTile + i;
+        if (j >= ntiles || key >= k1) return;
+        const int id = table[key >> 4];
+        if (id < 0 || id >= p.cache_blocks) return;
+        const long pb = 16L * D + kScaleBytes;
+        const uint8_t* at = cache + ((long)id * 2 * p.kv_heads + kvh) * pb + 16 * D + (key & 15) * 4;
+        ks = __ldg(reinterpret_cast<const float*>(at));
+        vs_ = __ldg(reinterpret_cast<const float*>(at + p.kv_heads * pb));
+      };
+      if constexpr (kQ) fetch(0);
+      bool odd = false;
+      for (int j = 0; j < ntiles; ++j) {
+        const int vs = j & 1, kb = k0 + j * kTile;
+        const bool inner = kb + kTile <= min(seg.cached, k1);
+        uint8_t* vt = smem + C::kOffV + vs * C::kTile16;
+        if constexpr (kQ) {
+          // The V stage's last reader (tile j - 2) is done, and with it the slot's (tile j - 4).
+          if (j >= 2 && !warp_wait(v_empty + vs, (j / 2 + 1) & 1, p.status, kTimeoutTmemEmpty, abort)) break;
+          const int slot = j % kSlots;
+          float* sk = scales + slot * 2 * kTile;
+          const uint32_t mine = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs_, 0.f)));
+          sk[i] = ks;
+          sk[kTile + i] = vs_;
+          // Each warp's largest V scale, by its bits (scales are not negative).
+          if (lane == 0) exps[slot * 4 + (i >> 5)] = (int)mine;
+          mbar_arrive(c_full + slot);
+          fetch(j + 1);
+        }
+        if (!warp_wait(v_land + vs, (j / 2) & 1, p.status, kTimeoutTmaFull, abort)) break;
+        if constexpr (kQ) {
+          const uint32_t raw = smem_u32(smem + C::kOffRaw + vs * C::kTile8);
+          const uint32_t dst = smem_u32(vt);
+          constexpr int kCh = D / 16;
+          auto convert = [&](const uint32_t (&w)[4], int key, int rc) {
+            const uint4 lo = make_uint4(e4m3x2_f16x2(w[0]), e4m3x2_f16x2_hi(w[0]), e4m3x2_f16x2(w[1]), e4m3x2_f16x2_hi(w[1]));
+            const uint4 hi = make_uint4(e4m3x2_f16x2(w[2]), e4m3x2_f16x2_hi(w[2]), e4m3x2_f16x2(w[3]), e4m3x2_f16x2_hi(w[3]));
+            // Lanes of the upper half of the columns store their chunks in the other order, so
+            // that a store's lanes fall in different banks.
+            const bool swap = kCh > 4 && rc >= 4;
+            sts128(dst + at16(key, 2 * rc + (swap ? 1 : 0)), swap ? hi : lo);
+            sts128(dst + at16(key, 2 * rc + (swap ? 0 : 1)), swap ? lo : hi);
+          };
+          if (inner) {
+#pragma unroll 2
+            for (int u = i; u < kTile * kCh; u += 128) {
+              const uint4 x = lds128(raw + at8<D>(u / kCh, u % kCh));
+              const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+              convert(w, u / kCh, u % kCh);
+            }
+          } else {
+#pragma unroll 1
+            for (int u = i; u < kTile * kCh; u += 128) {
+              const int key = u / kCh;
+              const uint4 x = lds128(raw + at8<D>(key, u % kCh));
+              uint32_t w[4] = {x.x, x.y, x.z, x.w};
+              if (kb + key >= seg.cached) {
+                // A product with a zero weight must stay zero.
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  if (kb + key >= k1) w[e] = 0u;
+#pragma unroll 1
+                  for (int y = 0; y < 32; y += 8)
+                    if ((w[e] >> y & 0x7fu) == 0x7fu) {
+                      w[e] &= ~(0xffu << y);
+                      odd = true;
+                    }
+                }
+              }
+              convert(w, key, u % kCh);
+            }
+          }
+          mbar_arrive(r_empty + vs);
+        } else if (!inner) {
+          const uint32_t dst = smem_u32(vt);
+          constexpr int kCh = D / 8;
+          for (int u = i; u < kTile * kCh; u += 128) {
+            const int key = u / kCh;
+            if (kb + key < seg.cached) continue;
+            const uint32_t a = dst + at16(key, u % kCh);
+            uint4 x = lds128(a);
+            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            bool change = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t bad = 0u;
+              if (kb + key >= k1) {
+                bad = ~0u;
+              } else {
+                if ((w[e] & 0x7f80u) == 0x7f80u) bad |= 0xffffu;
+                if ((w[e] & 0x7f800000u) == 0x7f800000u) bad |= 0xffff0000u;
+                if (bad != 0u) odd = true;
+              }
+              change = change || bad != 0u;
+              w[e] &= ~bad;
+            }
+            if (change) sts128(a, make_uint4(w[0], w[1], w[2], w[3]));
+          }
+        }
+        if (odd) atomicExch(odd_v, 1);
+        fence_proxy_async();
+        mbar_arrive(v_full + vs);
       }
     }
   }
