@@ -102,8 +102,11 @@ struct LogitsArgs {
   long ld_allowed = 0;
   int32_t* index = nullptr;  // -1 where no token is left
   float* value = nullptr;
+  float2* partial = nullptr;  // rows * logits_slices(vocab), when that is more than one a row
+  size_t partial_count = 0;
   int* status = nullptr;
 };
+int logits_slices(int vocab);
 int process_logits(const LogitsArgs& args, cudaStream_t stream);
 
 }  // namespace foa

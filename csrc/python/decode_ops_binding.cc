@@ -86,12 +86,13 @@ void bind_decode_ops(py::module_& m) {
     a.status = at<int>(status);
     check(foa::tree_attention(a, at<CUstream_st>(stream)), "tree_attention");
   }, py::call_guard<py::gil_scoped_release>());
+  m.def("logits_slices", &foa::logits_slices);
   m.def("process_logits", [](uint64_t logits, long ld, uint64_t out, long ldo, bool half, int rows, int vocab,
                              uint64_t prompt, uint64_t prompt_starts, int prompt_count, uint64_t output,
                              uint64_t output_starts, int output_count, uint64_t bias, uint64_t bias_starts,
                              int bias_count, uint64_t bias_values, uint64_t repetition, uint64_t frequency,
                              uint64_t presence, uint64_t allowed, long ld_allowed, uint64_t index, uint64_t value,
-                             uint64_t status, uint64_t stream) {
+                             uint64_t partial, size_t partial_count, uint64_t status, uint64_t stream) {
     foa::LogitsArgs a;
     a.logits = at<const void>(logits);
     a.out = at<void>(out);
@@ -111,6 +112,8 @@ void bind_decode_ops(py::module_& m) {
     a.ld_allowed = ld_allowed;
     a.index = at<int32_t>(index);
     a.value = at<float>(value);
+    a.partial = at<float2>(partial);
+    a.partial_count = partial_count;
     a.status = at<int>(status);
     check(foa::process_logits(a, at<CUstream_st>(stream)), "process_logits");
   }, py::call_guard<py::gil_scoped_release>());

@@ -315,10 +315,13 @@ def process_logits(logits, prompt=None, output=None, repetition=None, frequency=
             return index, value
         ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
         size = lambda t: 0 if t is None else t.numel()  # noqa: E731
-        native().ops.process_logits(
+        ops = native().ops
+        slices = ops.logits_slices(vocab)
+        partial = torch.empty(rows * slices, 2, dtype=torch.float32, device=logits.device) if slices > 1 else None
+        ops.process_logits(
             logits.data_ptr(), logits.stride(0), ptr(out), 0 if out is None else out.stride(0),
             logits.dtype == torch.bfloat16, rows, vocab, ptr(prompt_t), ptr(prompt_s), size(prompt_t), ptr(output_t),
             ptr(output_s), size(output_t), ptr(bias_t), ptr(bias_s), size(bias_t), ptr(values), ptr(repetition),
             ptr(frequency), ptr(presence), ptr(allowed), 0 if allowed is None else allowed.stride(0), index.data_ptr(),
-            value.data_ptr(), at.status, at.stream)
+            value.data_ptr(), ptr(partial), rows * slices, at.status, at.stream)
     return index, value
