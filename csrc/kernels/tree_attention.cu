@@ -661,7 +661,13 @@ int launch(const TreeAttention& p, cudaStream_t stream) {
   if (ctas > 2147483647L) return -2;
   constexpr int smem = Shape<D, kQ, NT>::kSmem;
   const auto kernel = tree_attention_kernel<D, kQ, NT>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -5;
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!configured[dev & 63]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -5;
+    configured[dev & 63] = true;
+  }
   if (launch_pdl(kernel, dim3((unsigned)ctas, splits), dim3(32 * kWarps), smem, stream, p, (int)mtiles, splits) != cudaSuccess)
     return -5;
   return merge<D>(p, splits, stream);

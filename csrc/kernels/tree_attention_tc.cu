@@ -860,7 +860,13 @@ int launch(const TreeAttention& p, int splits, cudaStream_t stream) {
                            CU_TENSOR_MAP_SWIZZLE_128B))
     return -4;
   const auto kernel = tree_attention_tc_kernel<D, kQ>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess) return -5;
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!configured[dev & 63]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess) return -5;
+    configured[dev & 63] = true;
+  }
   return launch_pdl(kernel, dim3((unsigned)ctas, splits), dim3(kThreads), C::kSmem, stream, maps, p, (int)mtiles, splits,
                     (int)pages) == cudaSuccess
              ? 0

@@ -9,6 +9,7 @@ import torch
 
 _lock = threading.Lock()
 _native = None
+_calls = None
 
 
 def native():
@@ -21,6 +22,19 @@ def native():
     return _native
 
 
+def calls():
+    """The ``_calls`` module (kernels called on torch tensors), connected to the native extension;
+    raises ImportError when either is not built."""
+    global _calls
+    if _calls is None:
+        with _lock:
+            if _calls is None:
+                module = importlib.import_module("furiosa_opt_models_b200.ops._calls")
+                module.connect(*importlib.import_module("furiosa_opt_engine._native").ops.decode_launchers())
+                _calls = module
+    return _calls
+
+
 class Scratch:
     """Device scratch of one GPU: split-K partials, arrival counters (kept zero between launches)
     and the status word kernels write instead of hanging."""
@@ -30,6 +44,7 @@ class Scratch:
         self.workspace = torch.empty(workspace_bytes // 4, dtype=torch.float32, device=device)
         self.counters = torch.zeros(counters, dtype=torch.int32, device=device)
         self.status = torch.zeros(4, dtype=torch.int32, device=device)
+        self.status_ptr = self.status.data_ptr()
 
     def check(self) -> None:
         """Raises RuntimeError when a kernel recorded a failure since the last check."""

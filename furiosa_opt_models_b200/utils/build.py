@@ -1,5 +1,6 @@
 """Builds the native engine: every CUDA kernel for sm_100a and the C++ host engine, linked into
-one in-tree extension, ``furiosa_opt_engine/_native*.so``.
+one in-tree extension, ``furiosa_opt_engine/_native*.so``; beside it the small module that calls
+kernels on torch tensors, ``furiosa_opt_models_b200/ops/_calls*.so``.
 
 The build is a generated ninja file under ``_build/`` so that a rebuild recompiles only what
 changed. ``nvcc`` cross-compiles for sm_100a without a GPU, so the build runs on any host with the
@@ -12,6 +13,7 @@ Usage: ``python -m furiosa_opt_models_b200.utils.build [--verbose] [--jobs N]``.
 from __future__ import annotations
 
 import argparse
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -34,6 +36,18 @@ def _pybind_include() -> str:
 
 def extension_path() -> Path:
     return ROOT / "furiosa_opt_engine" / ("_native" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def calls_path() -> Path:
+    """The module that calls kernels on torch tensors (built against torch, unlike the engine)."""
+    return ROOT / "furiosa_opt_models_b200" / "ops" / ("_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def _torch_dir() -> Path:
+    spec = importlib.util.find_spec("torch")
+    if spec is None or spec.origin is None:
+        raise RuntimeError("torch is needed to build the kernels' torch calls")
+    return Path(spec.origin).parent
 
 
 def _sources() -> tuple[list[Path], list[Path]]:
@@ -62,6 +76,15 @@ def _ninja_file(cu: list[Path], cc: list[Path]) -> str:
         "  command = g++ $ccflags -MMD -MF $out.d -c $in -o $out",
         "  depfile = $out.d",
         "  description = g++ $in",
+        "rule torch_cc",
+        f"  command = g++ -O2 -std=c++17 -fPIC -fvisibility=hidden -I{CSRC} -I{CSRC / 'kernels'} "
+        f"-isystem {_torch_dir() / 'include'} -isystem {_torch_dir() / 'include/torch/csrc/api/include'} "
+        f"-isystem {CUDA_HOME / 'include'} -I{sysconfig.get_paths()['include']} -MMD -MF $out.d -c $in -o $out",
+        "  depfile = $out.d",
+        "  description = g++ $in",
+        "rule torch_link",
+        f"  command = g++ -shared -o $out $in -L{_torch_dir() / 'lib'} -ltorch_python -ltorch_cpu -lc10 -lc10_cuda",
+        "  description = link $out",
         "rule link",
         "  command = g++ -o $out $in $ldflags",
         "  description = link $out",
@@ -78,7 +101,10 @@ def _ninja_file(cu: list[Path], cc: list[Path]) -> str:
         objs.append(obj)
         lines.append(f"build {obj}: cc {src}")
     lines.append(f"build {extension_path()}: link {' '.join(str(o) for o in objs)}")
-    lines.append(f"default {extension_path()}")
+    calls = BUILD / "obj" / "torch_decode_ops.o"
+    lines.append(f"build {calls}: torch_cc {CSRC / 'torch' / 'decode_ops.cc'}")
+    lines.append(f"build {calls_path()}: torch_link {calls}")
+    lines.append(f"default {extension_path()} {calls_path()}")
     return "\n".join(lines) + "\n"
 
 
