@@ -119,7 +119,10 @@ struct Page {
   static constexpr int kRow = kQ ? D : 2 * D;  // bytes of a key's row
   static constexpr int kChunks = kRow / 16;    // 16-byte chunks of a row
   static constexpr int kCodes = 16 * kRow;
-  static constexpr int kBytes = kCodes + (kQ ? kScaleBytes : 0);  // in the cache and in shared memory
+  static constexpr int kBytes = kCodes + (kQ ? kScaleBytes : 0);  // in the cache
+  // In shared memory: pages begin where an XOR of an address's swizzled bits is one of its offset's.
+  static constexpr int kAlign = kRow >= 128 ? kRow : 128;
+  static constexpr int kSlot = (kBytes + kAlign - 1) / kAlign * kAlign;
   static __device__ __forceinline__ uint32_t at(int r, int c) {
     int x;
     if constexpr (kChunks >= 8)
@@ -127,6 +130,10 @@ struct Page {
     else
       x = (r >> 1) & 3;  // 64-byte rows: two rows fill the banks
     return (uint32_t)(r * kRow + ((c ^ x) << 4));
+  }
+  // Chunk lane + 32 i of the page lies at (at(lane / kChunks, lane % kChunks) ^ flip(i)) + 512 i.
+  static __device__ __forceinline__ constexpr uint32_t flip(int i) {
+    return kChunks == 16 ? (uint32_t)(i & 3) << 4 : kChunks == 8 ? (uint32_t)(i & 1) << 5 : 0u;
   }
 };
 
@@ -150,9 +157,11 @@ __device__ __forceinline__ bool sees(const TreeAttention& p, const Segment& s, i
 // ------------------------------------------------------------------------------------ main kernel
 template <int D, bool kQ, int NT>
 struct Shape {
-  static constexpr int kStages = kQ ? 3 : 2;
-  static constexpr int kCtas = NT == 1 ? (kQ ? 4 : 3) : 2;  // of an SM, by registers and shared memory
-  static constexpr int kSmem = kWarps * kStages * 2 * Page<D, kQ>::kBytes;
+  // Two stages and many warps rather than three and fewer: what a warp waits for is mostly its own
+  // last instruction, not memory.
+  static constexpr int kStages = 2;
+  static constexpr int kCtas = NT == 1 ? (kQ ? 5 : 3) : (kQ ? 3 : 2);  // of an SM, by registers and shared memory
+  static constexpr int kSmem = kWarps * kStages * 2 * Page<D, kQ>::kSlot;
 };
 
 template <int D, bool kQ, int NT>
@@ -160,7 +169,7 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
     tree_attention_kernel(const TreeAttention p, int mtiles, int max_splits) {
   using P = Page<D, kQ>;
   constexpr int kStages = Shape<D, kQ, NT>::kStages;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(256) uint8_t smem[];
   constexpr int kSteps = D / 16;  // 16-wide k-steps of K Q^T, and 16-row tiles of O^T
   constexpr int kRows = 8 * NT;
   const int G = p.q_heads / p.kv_heads;
@@ -194,7 +203,7 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
   const int k0 = split * p.keys_per_split;
   const int k1 = min(keys, k0 + p.keys_per_split);
 
-  const uint32_t wbase = smem_u32(smem) + warp * kStages * 2 * P::kBytes;
+  const uint32_t wbase = smem_u32(smem) + warp * kStages * 2 * P::kSlot;
   const uint8_t* cache = static_cast<const uint8_t*>(p.cache);
   const int32_t* table = p.table + seg.table_start;
   const int b_last = (k1 - 1) / 16;
@@ -203,6 +212,9 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
   int ids = 0, ids_at = b_first;
   if (b_first + lane * kWarps <= b_last) ids = table[b_first + lane * kWarps];
 
+  const uint8_t* from = cache + (long)kvh * P::kBytes + lane * 16;
+  const uint32_t block = (uint32_t)(2 * p.kv_heads * P::kBytes), v_off = (uint32_t)(p.kv_heads * P::kBytes);
+  const uint32_t to = P::at(lane / P::kChunks, lane % P::kChunks);
   auto issue = [&](int b, int stage) {
     if (b >= ids_at + 32 * kWarps) {
       ids_at = b;
@@ -215,16 +227,14 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
       if (lane == 0) record_status(p.status, kBadIndex);
       id = 0;
     }
-    const uint8_t* kp = cache + ((long)id * 2 * p.kv_heads + kvh) * P::kBytes + lane * 16;
-    const uint8_t* vp = kp + (long)p.kv_heads * P::kBytes;
-    const uint32_t kt = wbase + stage * 2 * P::kBytes, vt = kt + P::kBytes;
+    const uint8_t* kp = from + (uint64_t)id * block;
+    const uint8_t* vp = kp + v_off;
+    const uint32_t kt = wbase + stage * 2 * P::kSlot, vt = kt + P::kSlot;
     const int n = valid ? 16 : 0;
 #pragma unroll
     for (int i = 0; i < (16 * P::kChunks) / 32; ++i) {
-      const int chunk = lane + i * 32;
-      const uint32_t dst = P::at(chunk / P::kChunks, chunk % P::kChunks);
-      cp_async16(kt + dst, kp + i * 512, n);
-      cp_async16(vt + dst, vp + i * 512, n);
+      cp_async16(((kt + to) ^ P::flip(i)) + i * 512, kp + i * 512, n);
+      cp_async16(((vt + to) ^ P::flip(i)) + i * 512, vp + i * 512, n);
     }
     if constexpr (kQ) {
       if (lane < 4) {
@@ -303,6 +313,9 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
   float v_lim = 0x1p-125f;     // 2^(v_exp + 1)
   bool odd_v = false;          // this lane left values that are not finite out of the products
 
+  // Addresses of this lane's fragments in a page; others of them differ in swizzled bits alone.
+  const uint32_t k_at = P::at(g, t);
+  const uint32_t v_at = kQ ? P::at(lane & 15, lane >> 4) : P::at((lane & 7) + 8 * (lane >> 4), lane >> 3 & 1);
   int stage = 0;
   for (int b = b_first; b <= b_last; b += kWarps, stage = stage + 1 == kStages ? 0 : stage + 1) {
     const int ahead = b + (kStages - 1) * kWarps;
@@ -312,7 +325,7 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
       cp_async_commit();
     cp_async_wait<kStages - 1>();
     __syncwarp();
-    const uint32_t kt = wbase + stage * 2 * P::kBytes, vt = kt + P::kBytes;
+    const uint32_t kt = wbase + stage * 2 * P::kSlot, vt = kt + P::kSlot;
     const bool inner = b * 16 + 16 <= min(seg.cached, k1);  // every row sees every key of the page
     if (!inner) {
       // A product with a zero weight must stay zero: rows past the keys are cleared, and values
@@ -358,7 +371,8 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
     if constexpr (kQ) {
 #pragma unroll
       for (int h = 0; h < kSteps / 4; ++h) {
-        const uint4 x = lds128(kt + P::at(g, t + 4 * h)), y = lds128(kt + P::at(g + 8, t + 4 * h));
+        const uint32_t at = (kt + k_at) ^ (h << 6);
+        const uint4 x = lds128(at), y = lds128(at + 8 * P::kRow);
         const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -370,7 +384,8 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
     } else {
 #pragma unroll
       for (int h = 0; h < kSteps / 2; ++h) {
-        const uint4 x = lds128(kt + P::at(g, t + 4 * h)), y = lds128(kt + P::at(g + 8, t + 4 * h));
+        const uint32_t at = (kt + k_at) ^ (h << 6);
+        const uint4 x = lds128(at), y = lds128(at + 8 * P::kRow);
         const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -473,7 +488,7 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
 #pragma unroll
       for (int c = 0; c < P::kChunks; c += 2) {
         uint32_t r[4];
-        ldsm_x4_t(r, vt + P::at(lane & 15, c + (lane >> 4)));
+        ldsm_x4_t(r, (vt + v_at) ^ (c << 4));
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           const uint32_t lo = __byte_perm(r[2 * w], 0u, 0x3120), hi = __byte_perm(r[2 * w + 1], 0u, 0x3120);
@@ -487,7 +502,7 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
 #pragma unroll
       for (int c = 0; c < kSteps; ++c) {
         uint32_t r[4];
-        ldsm_x4_t(r, vt + P::at((lane & 7) + 8 * (lane >> 4), 2 * c + (lane >> 3 & 1)));
+        ldsm_x4_t(r, (vt + v_at) ^ (2 * c << 4));
 #pragma unroll
         for (int n = 0; n < NT; ++n) mma_b16(o[n][c], r, pb[n][0], pb[n][1]);
       }
@@ -696,7 +711,7 @@ int tree_attention_split(int num_segments, int q_heads, int kv_heads, int head_d
   const long items = (rows + tile - 1) / tile * kv_heads * num_segments;
   // About two (tcgen05) or four CTAs for each that the GPU holds at once, of at least so many keys
   // that a CTA's start and end do not count.
-  const long want = tc ? 148L * 2 : 148L * 4 * 2;
+  const long want = tc ? 148L * 2 : 148L * 4 * 4;
   const long least = tc ? 512 : 256;
   const long per = ((long)max_keys * items + want - 1) / want;
   const long keys = ((per < least ? least : per) + 127) / 128 * 128;
