@@ -613,6 +613,56 @@ def test_process_logits_ties_in_place_and_bad_lists():
     assert none[0].shape == (0,)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab,output,biases,padding", [
+    (2, 20000, 30000, 9000, 0),  # most of the vocabulary listed
+    (900, 8200, 40, 3, 0),       # more slices than the GPU holds at once
+    (3, 9000, 4000, 3000, 1 << 21),  # lists whose counts and places need more than one word
+])
+def test_process_logits_long_lists_in_place(rows, vocab, output, biases, padding, dtype):
+    ops = _ops()
+    gen = torch.Generator().manual_seed(vocab)
+    x = torch.randn(rows, vocab, generator=gen).mul(4).to(dtype)
+    draw = lambda n: torch.randint(0, vocab, (rows, n), generator=gen)  # noqa: E731
+    prompt, out_tokens = draw(output // 2), draw(output)
+    out_tokens[0, : output // 2] = 5  # one token many times
+    bias_tokens = torch.stack([torch.randperm(vocab, generator=gen)[:biases] for _ in range(rows)])
+    bias_values = torch.randn(rows, biases, generator=gen)
+    rep = torch.rand(rows, generator=gen) + 0.8
+    freq, pres = torch.rand(rows, generator=gen) * 0.1, torch.rand(rows, generator=gen)
+    allowed = torch.rand(rows, vocab, generator=gen) < 0.6
+
+    def csr(tokens, extra=0):
+        flat = torch.cat([tokens.flatten().to(I32), torch.full((extra,), vocab, dtype=I32)])
+        return flat.to(DEV), (torch.arange(rows + 1) * tokens.shape[1]).to(I32).to(DEV)
+
+    bt, bs = csr(bias_tokens)
+    kw = dict(prompt=csr(prompt), output=csr(out_tokens, padding), repetition=rep.to(DEV), frequency=freq.to(DEV),
+              presence=pres.to(DEV), bias=(bt, bias_values.flatten().to(DEV), bs), allowed=_bits(allowed))
+    mine = x.to(DEV)
+    index, value = ops.process_logits(mine, out=mine, **kw)
+    _check()
+    count = torch.zeros(rows, vocab, dtype=torch.float64).scatter_add_(1, out_tokens, torch.ones(rows, output, dtype=torch.float64))
+    listed = (count > 0).scatter(1, prompt, torch.ones(rows, output // 2, dtype=torch.bool))
+    col = lambda v: v.double()[:, None]  # noqa: E731
+    ref = x.double()
+    size = ref.abs()
+    ref = torch.where(listed, torch.where(ref > 0, ref / col(rep), ref * col(rep)), ref)
+    size = size + ref.abs() + (count > 0) * (col(freq) * count + col(pres))
+    ref = ref - (count > 0) * (col(freq) * count + col(pres))
+    ref = ref.scatter_add(1, bias_tokens, bias_values.double())
+    size = size.scatter_add(1, bias_tokens, bias_values.double().abs())
+    # Five FP32 steps, and one rounding of the stored logit.
+    tol = 5 * 2.0 ** -24 * size
+    got = mine.double().cpu()
+    assert torch.equal(got == -torch.inf, ~allowed)
+    assert ((got - ref).abs() <= tol + (_half(BF16) * ref.abs() if dtype == BF16 else 0))[allowed].all()
+    i, row = index.long().cpu(), torch.arange(rows)
+    assert allowed[row, i].all() and ((value.double().cpu() - ref[row, i]).abs() <= tol[row, i]).all()
+    least = torch.where(allowed, ref - tol, torch.tensor(-torch.inf, dtype=torch.float64)).amax(1)
+    assert (ref[row, i] + tol[row, i] >= least).all()
+
+
 # ------------------------------------------------------------------------------- a run of them all
 
 
