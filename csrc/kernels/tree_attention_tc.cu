@@ -36,8 +36,6 @@ namespace foa {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLift = 10.f;   // weights are scaled by 2^10 ...
-constexpr float kSlack = 4.f;   // ... and may exceed the row's reference maximum by 2^4
 constexpr int kLeastExp = -90;  // least exponent of V's reference scale (sums stay below 2^127)
 constexpr int kTile = 128;      // rows and keys of an MMA tile
 constexpr int kThreads = 512;   // 8 softmax warps, MMA, loader, 4 helpers, 2 idle (whole warpgroups)
@@ -48,6 +46,7 @@ constexpr int kSlots = 4;       // key tiles whose scales are held
 
 template <int D, bool kQ>
 struct Cfg {
+  static constexpr float kLift = kQ ? 6.f : 0.f, kSlack = kQ ? 8.f : 14.f;
   static constexpr int kHalf = kTile * 128;            // a tile's 64 16-bit columns
   static constexpr int kTile16 = kTile * D * 2;        // a 16-bit tile
   static constexpr int kTile8 = kTile * D;             // an 8-bit tile
@@ -397,18 +396,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     int i = 0;
     for (int n = w; n < steps; n += 2, ++i) {
       const int j = two ? i : n, kb = k0 + j * kTile;
-      if (!warp_wait(s_full + w, i & 1, p.status, kTimeoutTmemFull, abort)) {
+      const int slot = j % kSlots;
+      // (A wait costs some 200 cycles even for what is there: the last to come is waited for last.)
+      if ((kQ && !warp_wait(c_full + slot, (j / kSlots) & 1, p.status, kTimeoutTmemFull, abort)) ||
+          !warp_wait(s_full + w, i & 1, p.status, kTimeoutTmemFull, abort)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      const int slot = j % kSlots;
-      if constexpr (kQ) {
-        if (!warp_wait(c_full + slot, (j / kSlots) & 1, p.status, kTimeoutTmemFull, abort)) {
-          ok = false;
-          break;
-        }
-      }
       if (!idle) {
         const float* sk = scales + slot * 2 * kTile;
         const bool inner = kb + kTile <= min(seg.cached, k1);
@@ -460,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         float mx = fmaxf(mx0, mx1), f = 1.f;
         if (mx > -INFINITY) mx *= c;
-        if (mx > top + kSlack) {
+        if (mx > top + C::kSlack) {
           f = top == -INFINITY ? 0.f : ex2(top - mx);
           top = mx;
         }
@@ -481,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_st_32x32b_x16(o_col + c0, y);
           }
         }
-        const float z = top == -INFINITY ? 0.f : top + (float)v_exp - kLift;
+        const float z = top == -INFINITY ? 0.f : top + (float)v_exp - C::kLift;
         const float2 c2 = make_float2(c, c), z2 = make_float2(-z, -z);
         float2 acc0 = make_float2(0.f, 0.f), acc1 = acc0;
         // P takes the columns of S.
@@ -642,17 +637,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
       };
-      int got_k = 0, got_v = 0, next = page_of(0);
-      for (int j = 0; j < ntiles; ++j) {
-        const int ks = j % C::kKStages, vs = j & 1, page = next;
-        if (j >= C::kKStages && !warp_wait(k_empty + ks, (j / C::kKStages + 1) & 1, p.status, kTimeoutSmemEmpty, abort)) break;
+      int got_k = 0, got_v = 0;
+      auto load_k = [&](int j, int page) {
+        const int ks = j % C::kKStages;
+        if (j >= C::kKStages && !warp_wait(k_empty + ks, (j / C::kKStages + 1) & 1, p.status, kTimeoutSmemEmpty, abort)) return false;
         load(smem + C::kOffK + ks * C::kKStage, k_full + ks, page);
         ++got_k;
-        next = page_of(j + 1);
+        return true;
+      };
+      // K runs two tiles ahead of V: the S of tile j + 2 is issued behind the P V of tile j.
+      int page0 = page_of(0), page1 = page_of(1), page2 = page_of(2);
+      load_k(0, page0);
+      if (ntiles > 1) load_k(1, page1);
+      for (int j = 0; j < ntiles; ++j) {
+        const int vs = j & 1;
         if (j >= 2 && !warp_wait((kQ ? r_empty : v_empty) + vs, (j / 2 + 1) & 1, p.status, kTimeoutSmemEmpty, abort)) break;
         load(smem + (kQ ? C::kOffRaw + vs * C::kTile8 : C::kOffV + vs * C::kTile16), v_land + vs,
-             page == num_pages ? num_pages : page + p.kv_heads);
+             page0 == num_pages ? num_pages : page0 + p.kv_heads);
         ++got_v;
+        if (j + 2 < ntiles && !load_k(j + 2, page2)) break;
+        page0 = page1;
+        page1 = page2;
+        page2 = page_of(j + 3);
       }
       // Let the loads in flight land before the CTA may exit (an abort stops the loop early).
       for (int j = got_k > C::kKStages ? got_k - C::kKStages : 0; j < got_k; ++j)
@@ -665,11 +671,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr uint32_t idesc_s = kQ ? idesc_e4m3_f32(kTile, kTile) : idesc_bf16_f32(kTile, kTile);
         // P V: FP16 (format 0) over codes, BF16 else; B (V) MN-major.
         constexpr uint32_t idesc_o = (kQ ? idesc_bf16_f32(kTile, D) & ~((1u << 7) | (1u << 10)) : idesc_bf16_f32(kTile, D)) | (1u << 16);
-        bool ok = wait1(q_full, 0, p.status, kTimeoutTmemFull, abort);
-        auto scores = [&](int n) -> bool {
+        const bool ok = wait1(q_full, 0, p.status, kTimeoutTmemFull, abort);
+        auto scores = [&](int n) {
           const int w = n & 1, j = two ? n >> 1 : n, ks = j % C::kKStages;
-          if (!wait1(k_full + ks, (j / C::kKStages) & 1, p.status, kTimeoutTmaFull, abort)) return false;
-          tc_fence_after();
           // (Descriptors of a tile's steps differ in their address field alone.)
           const uint8_t* kt = smem + C::kOffK + ks * C::kKStage;
           const uint8_t* qt = smem + C::kOffQ + (two ? w : 0) * C::kQTile;
@@ -691,13 +695,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           mma_commit(s_full + w);
           if (!two || w == 1) mma_commit(k_empty + ks);
-          return true;
         };
         for (int n = -2; ok && n < steps; ++n) {
+          const int w = n & 1, jk = two ? (n + 2) >> 1 : n + 2;
+          if (n + 2 < steps && !wait1(k_full + jk % C::kKStages, (jk / C::kKStages) & 1, p.status, kTimeoutTmaFull, abort)) break;
           if (n >= 0) {
-            const int w = n & 1, j = two ? n >> 1 : n, vs = j & 1;
-            if (!wait1(p_full + w, (n >> 1) & 1, p.status, kTimeoutTmemFull, abort) ||
-                !wait1(v_full + vs, (j / 2) & 1, p.status, kTimeoutTmaFull, abort))
+            const int j = two ? n >> 1 : n, vs = j & 1;
+            if (!wait1(v_full + vs, (j / 2) & 1, p.status, kTimeoutTmaFull, abort) ||
+                !wait1(p_full + w, (n >> 1) & 1, p.status, kTimeoutTmemFull, abort))
               break;
             tc_fence_after();
             const uint64_t vd = desc_mn16(smem + C::kOffV + vs * C::kTile16, C::kHalf, 1024);
@@ -707,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                          n >= 2 || kk > 0 ? 1u : 0u);
             if (!two || w == 1) mma_commit(v_empty + vs);
           }
-          if (n + 2 < steps) ok = scores(n + 2);
+          if (n + 2 < steps) scores(n + 2);
         }
         // No MMA may still write TMEM when it is read or freed (an abort can leave some in flight).
         mma_commit(done);
