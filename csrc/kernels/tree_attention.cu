@@ -308,9 +308,12 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
     m_[n][0] = m_[n][1] = -INFINITY;
     l_[n][0] = l_[n][1] = 0.f;
   }
-  int v_exp = -126;            // exponent of the largest V scale of the pages so far
-  float v_inv = 0x1p126f;      // 2^-v_exp
-  float v_lim = 0x1p-125f;     // 2^(v_exp + 1)
+  // 2^-e, e the exponent of the largest V scale that the row has seen (a drafted node's values may be
+  // far larger than those of rows that do not see it), and the least 2^(e + 1) of this lane's rows.
+  float v_inv[NT][2];
+  float v_lim = 0x1p-125f;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) v_inv[n][0] = v_inv[n][1] = 0x1p126f;
   bool odd_v = false;          // this lane left values that are not finite out of the products
 
   // Addresses of this lane's fragments in a page; others of them differ in swizzled bits alone.
@@ -429,16 +432,7 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
 #pragma unroll
       for (int i = 0; i < 2; ++i) move = move || fmaxf(s[n][i], s[n][i + 2]) > m_[n][i] + kSlack;
     if (__any_sync(0xffffffffu, move)) {
-      float fv = 1.f;
-      if constexpr (kQ) {
-        // (Scales are not negative: their bits order as they do.)
-        const uint32_t top = __reduce_max_sync(0xffffffffu, max(__float_as_uint(fmaxf(vs[0], 0.f)), __float_as_uint(fmaxf(vs[1], 0.f))));
-        const int e = max(v_exp, min(max((int)(top >> 23), 1), 253) - 127);
-        fv = ex2((float)(v_exp - e));
-        v_exp = e;
-        v_inv = __uint_as_float((uint32_t)(127 - e) << 23);  // e <= 126
-        v_lim = __uint_as_float((uint32_t)(128 + e) << 23);
-      }
+      v_lim = INFINITY;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -451,6 +445,18 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
           const float f = x == -INFINITY ? 1.f : ex2(m_[n][i] - x);
           m_[n][i] = x;
           l_[n][i] *= f;
+          float fv = 1.f;
+          if constexpr (kQ) {
+            float top = fmaxf(s[n][i] > -INFINITY ? vs[0] : 0.f, s[n][i + 2] > -INFINITY ? vs[1] : 0.f);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            const int was = 127 - (int)(__float_as_uint(v_inv[n][i]) >> 23);
+            const int e = max(was, min(max((int)(__float_as_uint(top) >> 23), 1), 253) - 127);
+            fv = ex2((float)(was - e));
+            v_inv[n][i] = __uint_as_float((uint32_t)(127 - e) << 23);  // e <= 126
+            v_lim = fminf(v_lim, __uint_as_float((uint32_t)(128 + e) << 23));
+          }
 #pragma unroll
           for (int c = 0; c < kSteps; ++c) {
             o[n][c][i] *= f * fv;
@@ -469,7 +475,7 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
         const float z = m_[n][i & 1] == -INFINITY ? 0.f : m_[n][i & 1] - kLift;
         w[i] = ex2(s[n][i] - z);
         l_[n][i & 1] += w[i];
-        if constexpr (kQ) w[i] *= vs[i >> 1] * v_inv;
+        if constexpr (kQ) w[i] *= !inner && s[n][i] == -INFINITY ? 0.f : vs[i >> 1] * v_inv[n][i & 1];
       }
       if constexpr (kQ) {
         pb[n][0] = transpose8(pack_f16x2(w[0], w[1]));
@@ -533,12 +539,12 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
         sm_l[warp * kRows + 8 * n + 2 * t + i] = l_[n][i];
       }
   }
-  const float back = kQ ? __uint_as_float((uint32_t)(127 + v_exp) << 23) : 1.f;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float* dst = sm_o + (warp * kRows + 8 * n + 2 * t + i) * D;
+      const float back = kQ ? __uint_as_float((254u << 23) - __float_as_uint(v_inv[n][i])) : 1.f;  // 2^e
 #pragma unroll
       for (int c = 0; c < kSteps; ++c) {
         if constexpr (kQ) {

@@ -441,6 +441,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!inner) {
           mx0 = mx1 = -INFINITY;
+          // V's reference is of the scales that the row sees: a drafted node's may be far larger.
+          float most = 0.f;
 #pragma unroll
           for (int c0 = 0; c0 < kTile; c0 += 32) {
             const uint32_t seen = visible(p, seg, tok, kb + c0, k1);
@@ -449,8 +451,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               const float t = seen >> x & 1u ? __uint_as_float(r[c0 + x]) : -INFINITY;
               r[c0 + x] = __float_as_uint(t);
               mx0 = fmaxf(mx0, t);
+              if constexpr (kQ) most = fmaxf(most, seen >> x & 1u ? sk[kTile + c0 + x] : 0.f);
             }
           }
+          if constexpr (kQ) e = max(v_exp, min((int)(__float_as_uint(most) >> 23), 253) - 127);
           __syncwarp();
         }
         float mx = fmaxf(mx0, mx1), f = 1.f;

@@ -363,6 +363,29 @@ def test_what_a_row_does_not_see_does_not_reach_it(n, quantized):
                 assert (out[r, :, 12] == float("inf")).all()
 
 
+@pytest.mark.parametrize("n", [3, 6, 70, 150])
+def test_a_large_value_stays_with_the_rows_that_see_it(n):
+    """A drafted node whose values are 2^100 times the others': its scale is no other row's unit."""
+    ops = _ops()
+    gen = torch.Generator().manual_seed(5)
+    hq, hk, d = 8, 2, 128
+    lens, cached = [n], [300]
+    cache, table, segs, values, tab, sl = _paged(lens, cached, hk, d, True, gen)
+    b, o = tab[302 // 16], 302 % 16  # node 2
+    values[b, 1, :, o] *= 2.0 ** 100
+    at = slice(16 * d + 4 * o, 16 * d + 4 * o + 4)
+    scale = cache.pages[b, 1, :, at].contiguous().view(F32) * 2.0 ** 100
+    cache.pages[b, 1, :, at] = scale.view(torch.uint8)
+    ms = [torch.eye(n, dtype=torch.bool)]
+    ms[0][n - 1, 0] = True
+    q = torch.randn(n, hq, d, generator=gen).to(BF16)
+    ref, weight, err = _attend64(q, values, tab, sl, d ** -0.5, mask=ms)
+    for split in (None, 16, 128):
+        out = ops.paged_tree(q.to(DEV), cache, table, segs, hk, n + 300, n, mask=_pack(ms), keys_per_split=split).cpu()
+        _check()
+        assert ((out.double() - ref).abs() <= _tolerance(ref, weight, err, d, True)).all()
+
+
 @pytest.mark.parametrize("quantized", [True, False], ids=["e4m3", "bf16"])
 def test_scores_of_a_wide_range(quantized):
     """Scores that rise by hundreds along the keys, and rows of large and of tiny queries."""
