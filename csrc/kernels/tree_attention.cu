@@ -18,13 +18,19 @@
 // the warps issue a page decides. The codes become FP16 exactly in registers (cvt.rn.f16x2.e4m3x2):
 // - Q is scaled a row by a power of two (exact) so that FP16 holds it; K's scales multiply S.
 // - V's scales multiply the weights before they round to FP16, by way of a power of two that keeps
-//   the largest scale seen near one; that and the rows' maxima move only when a page exceeds them
-//   (the maxima by 2^4), which one vote a page finds. Weights stay below 2^15 of FP16's 65504 and
-//   lose what lies 2^-34 below the largest.
+//   the largest scale that the row has seen near one; that and the rows' maxima move only when a page
+//   exceeds them (the maxima by 2^4), which one vote a page finds. Weights stay below 2^15 of FP16's
+//   65504 and lose what lies 2^-34 below the largest.
 // - K fragments are read 16 codes a lane: the MMA's k index runs over the head's elements in the
 //   order that makes each lane's codes contiguous (Q's fragments follow the same order). V
 //   fragments come from ldmatrix.trans over byte pairs, one prmt apart.
 // Sums and statistics are FP32; P rounds to FP16 (BF16 over a BF16 cache), o once to BF16.
+//
+// Bound by HBM for batches of long histories (64 uniform sequences of 8192 keys, 32 x 8 heads: 6100
+// GB/s over codes, 6800 over BF16), by uneven CTAs where lengths differ (64 sequences of 1152 to 9216
+// keys: 112 us, 5400 GB/s), by the chain of one CTA and the join for few (one of 1000 keys: 8.2 us).
+// Two pages in flight a warp and five CTAs an SM take 110 us where three pages, four CTAs and
+// addresses computed for each access take 123.
 
 #include "decode_ops.cuh"
 #include "launch.cuh"
@@ -604,11 +610,12 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
 
 // Joins the splits of each (row, head): a CTA each, whose warps take the splits in turn and meet in
 // a fixed order. (One warp a head took 20 us for 64 splits of 192 heads: it waits for one load
-// after another.)
-template <int D>
-__global__ void __launch_bounds__(128) tree_merge_kernel(const TreeAttention p, int max_splits) {
+// after another.) Few rows of many splits get sixteen warps: with four, one sequence of 131072 keys and
+// 16 heads in 256 splits took 77 us, with sixteen 60.
+template <int D, int W>
+__global__ void __launch_bounds__(32 * W) tree_merge_kernel(const TreeAttention p, int max_splits) {
   constexpr int E = D / 32;
-  __shared__ float sm_acc[3][D], sm_den[3];
+  __shared__ float sm_acc[W - 1][D], sm_den[W - 1];
   pdl_wait();
   pdl_trigger();
   const Segment seg = p.segments[blockIdx.x / p.max_len];
@@ -628,7 +635,7 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeAttention p, 
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
   if (top > -INFINITY) {
 #pragma unroll 4
-    for (int s = warp; s < nsplit; s += 4) {
+    for (int s = warp; s < nsplit; s += W) {
       const float2 ml = p.partial_ml[base + s];
       const float w = ex2(ml.x - top);
       den = fmaf(w, ml.y, den);
@@ -653,7 +660,7 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeAttention p, 
   __syncthreads();
   if (warp > 0) return;
 #pragma unroll
-  for (int w = 0; w < 3; ++w) {
+  for (int w = 0; w < W - 1; ++w) {
     den += sm_den[w];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] += sm_acc[w][lane * E + e];
@@ -667,10 +674,11 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeAttention p, 
 template <int D>
 int merge(const TreeAttention& p, int splits, cudaStream_t stream) {
   if (splits == 1) return 0;
-  return launch_pdl(tree_merge_kernel<D>, dim3(p.num_segments * p.max_len, p.q_heads), dim3(128), 0, stream, p, splits) ==
-                 cudaSuccess
-             ? 0
-             : -5;
+  const dim3 grid(p.num_segments * p.max_len, p.q_heads);
+  const bool few = splits > 16 && (long)p.num_segments * p.max_len * p.q_heads <= 148L * 8;
+  const cudaError_t rc = few ? launch_pdl(tree_merge_kernel<D, 16>, grid, dim3(512), 0, stream, p, splits)
+                                     : launch_pdl(tree_merge_kernel<D, 4>, grid, dim3(128), 0, stream, p, splits);
+  return rc == cudaSuccess ? 0 : -5;
 }
 
 template <int D, bool kQ, int NT>
@@ -715,10 +723,12 @@ int tree_attention_split(int num_segments, int q_heads, int kv_heads, int head_d
   const bool tc = tc_rows(max_len, (int)(q_heads / kv_heads));
   const long tile = tc ? 256 : 16;
   const long items = (rows + tile - 1) / tile * kv_heads * num_segments;
-  // About two (tcgen05) or four CTAs for each that the GPU holds at once, of at least so many keys
-  // that a CTA's start and end do not count.
-  const long want = tc ? 148L * 2 : 148L * 4 * 4;
-  const long least = tc ? 512 : 256;
+  // About two (tcgen05) or three CTAs for each that the GPU holds at once (segments may differ in
+  // length), of at least so many keys that a CTA's start and end do not count; fewer where the GPU is
+  // far from full (one sequence of 1000 keys, 8 heads: 8.2 us in splits of 128, 9.5 of 256; four of
+  // 2048: 11.4 and 10.8).
+  const long want = tc ? 148L * 2 : 148L * 16;
+  const long least = tc ? 512 : items * (((long)max_keys + 127) / 128) <= 148L * 2 ? 128 : 256;
   const long per = ((long)max_keys * items + want - 1) / want;
   const long keys = ((per < least ? least : per) + 127) / 128 * 128;
   return (int)(keys > max_keys ? (max_keys + 15) / 16 * 16 : keys);

@@ -16,13 +16,24 @@
 //   E4M3 would lose a long tail of small probabilities; they write the keys' scales beside it.
 // - BF16 pages: TMA brings K and V as the MMAs read them; the helpers only clear V rows past the
 //   keys and values that are not finite.
-// - Row maxima move when a tile exceeds them by 2^4, the reference exponent of V's scales when a
-//   tile's largest does; O is rescaled in TMEM then. Both are part of the unit that O and the row's
-//   sum are held in.
+// - Row maxima move when a tile exceeds them by 2^kSlack, the reference exponent of V's scales when the
+//   largest that the row sees does; O is rescaled in TMEM then, which takes 3000 cycles beside 3700 of a
+//   pair of tiles. With slack 2^4 that happened to a warp in every third tile early on; FP16 weights of
+//   slack 2^8 still hold 2^-20 of the reference in full and 2^-30 at all. Both are part of the unit that
+//   O and the row's sum are held in.
 // - Every wait is bounded; a timeout records a status and every role leaves through the same end.
 //
-// Over quantized pages with 256 rows the MMAs bound it (two FP8 passes of S cost what one FP16 pass
-// does), with 128 or fewer HBM does.
+// What bounds it: the chain of one warpgroup (128 scores a thread, P to TMEM, P V, the next S, which
+// overwrites P), overlapped with the other one's; over codes the shared-memory pipe beside it, since
+// every thread reads every key's two scales (a broadcast of 16 bytes takes as long as 512 bytes) while
+// the MMAs read Q, K and V there. 24 trees of 32 to 64 nodes over 4.5 to 16.4 thousand keys, 32 x 8
+// heads of 128: 460 us over codes, 335 over BF16 pages (590 TFLOP/s); 16 of 16 to 31 nodes: 127 and 120.
+// An mbarrier wait costs the MMA thread 200 cycles even for a phase long complete, so what is surely
+// there (K, V, scales) is waited for before what is not (P, S): 496 -> 462 us. Tried and slower, over
+// the same trees with the kernel of that day: S in halves of 64 keys so that S overlaps the softmax
+// (BF16 450 us for 336: N = 64 reads Q twice as often), K and V dequantized to FP16 by the helpers (530
+// for 502), two MMA threads (527), scores in fragments of 16 x 256 bits (534), weights in a rolled loop
+// of two passes (526).
 
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -46,6 +57,8 @@ constexpr int kSlots = 4;       // key tiles whose scales are held
 
 template <int D, bool kQ>
 struct Cfg {
+  // Weights are scaled by 2^kLift and may exceed the row's reference by 2^kSlack: below 2^15 over codes,
+  // where V's scale, under 2 in the reference's units, still multiplies them before they are FP16.
   static constexpr float kLift = kQ ? 6.f : 0.f, kSlack = kQ ? 8.f : 14.f;
   static constexpr int kHalf = kTile * 128;            // a tile's 64 16-bit columns
   static constexpr int kTile16 = kTile * D * 2;        // a 16-bit tile
@@ -391,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     const bool idle = !__any_sync(0xffffffffu, real);  // none of the warp's rows counts
     float top = -INFINITY, sum = 0.f;
-    int v_exp = kQ ? kLeastExp : 0;  // O and the sums are in units of 2^(top + v_exp - 10)
+    int v_exp = kQ ? kLeastExp : 0;  // O and the sums are in units of 2^(top + v_exp - kLift)
     bool ok = true;
     int i = 0;
     for (int n = w; n < steps; n += 2, ++i) {
