@@ -610,8 +610,9 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
 
 // Joins the splits of each (row, head): a CTA each, whose warps take the splits in turn and meet in
 // a fixed order. (One warp a head took 20 us for 64 splits of 192 heads: it waits for one load
-// after another.) Few rows of many splits get sixteen warps: with four, one sequence of 131072 keys and
-// 16 heads in 256 splits took 77 us, with sixteen 60.
+// after another.) Rows of more than sixteen splits get sixteen warps: with four, one sequence of 131072
+// keys and 16 heads in 256 splits took 77 us, with sixteen 60. How many take part follows from the
+// row's own splits, so that the order of its sums is the same in every call.
 template <int D, int W>
 __global__ void __launch_bounds__(32 * W) tree_merge_kernel(const TreeAttention p, int max_splits) {
   constexpr int E = D / 32;
@@ -624,6 +625,7 @@ __global__ void __launch_bounds__(32 * W) tree_merge_kernel(const TreeAttention 
   if (tok >= seg.len || !rows_fit(p, seg) || !segment_fits(p, seg)) return;
   const int nsplit = (seg.cached + seg.len + p.keys_per_split - 1) / p.keys_per_split;
   if (nsplit == 1) return;  // written in place
+  const int warps = nsplit > 16 ? 16 : 4;  // (the launch has sixteen when a row may need them)
   const long row = seg.row_start + tok;
   const long base = (row * p.q_heads + head) * max_splits;
   float top = -INFINITY;
@@ -635,7 +637,7 @@ __global__ void __launch_bounds__(32 * W) tree_merge_kernel(const TreeAttention 
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
   if (top > -INFINITY) {
 #pragma unroll 4
-    for (int s = warp; s < nsplit; s += W) {
+    for (int s = warp < warps ? warp : nsplit; s < nsplit; s += warps) {
       const float2 ml = p.partial_ml[base + s];
       const float w = ex2(ml.x - top);
       den = fmaf(w, ml.y, den);
@@ -661,6 +663,7 @@ __global__ void __launch_bounds__(32 * W) tree_merge_kernel(const TreeAttention 
   if (warp > 0) return;
 #pragma unroll
   for (int w = 0; w < W - 1; ++w) {
+    if (w + 1 >= warps) break;
     den += sm_den[w];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] += sm_acc[w][lane * E + e];
@@ -675,8 +678,7 @@ template <int D>
 int merge(const TreeAttention& p, int splits, cudaStream_t stream) {
   if (splits == 1) return 0;
   const dim3 grid(p.num_segments * p.max_len, p.q_heads);
-  const bool few = splits > 16 && (long)p.num_segments * p.max_len * p.q_heads <= 148L * 8;
-  const cudaError_t rc = few ? launch_pdl(tree_merge_kernel<D, 16>, grid, dim3(512), 0, stream, p, splits)
+  const cudaError_t rc = splits > 16 ? launch_pdl(tree_merge_kernel<D, 16>, grid, dim3(512), 0, stream, p, splits)
                                      : launch_pdl(tree_merge_kernel<D, 4>, grid, dim3(128), 0, stream, p, splits);
   return rc == cudaSuccess ? 0 : -5;
 }

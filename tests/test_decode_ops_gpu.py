@@ -463,6 +463,24 @@ def test_a_fixed_split_gives_the_same_bits_in_any_batch():
     assert torch.equal(whole[3], one[3])
 
 
+def test_a_long_row_of_many_splits_has_the_same_bits_in_any_batch():
+    ops = _ops()
+    gen = torch.Generator().manual_seed(8)
+    hq, hk, d = 16, 4, 64
+    lens, cached = [1] * 70, [16 * 40 - 1, 16 * 11 + 3] + [16 * 30] + [16 * (i % 19) + i % 7 for i in range(67)]
+    cache, table, segs, values, tab, sl = _paged(lens, cached, hk, d, True, gen)
+    q = torch.randn(70, hq, d, generator=gen).to(BF16).to(DEV)
+    every = ops.paged_decode(q, cache, table, segs, hk, max(cached) + 1, keys_per_split=16)
+    for i in range(4):
+        alone = segs[i:i + 1].clone()
+        alone[0, 0] = 0
+        one = ops.paged_decode(q[i:i + 1], cache, table, alone, hk, cached[i] + 1, keys_per_split=16)
+        assert torch.equal(one[0], every[i])
+    _check()
+    ref, weight, err = _attend64(q.cpu(), values, tab, sl, d ** -0.5)
+    assert ((every.double().cpu() - ref).abs() <= _tolerance(ref, weight, err, d, True)).all()
+
+
 def test_offsets_past_32_bits():
     """Pages beyond 2^32 bytes of the cache: a quantized cache of 4.6 GB whose last blocks are used."""
     ops = _ops()
