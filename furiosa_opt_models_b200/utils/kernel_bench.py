@@ -132,12 +132,76 @@ def decode_attn(args) -> dict:
     table = torch.arange(rows * nb, dtype=torch.int32, device="cuda")
     seg = torch.tensor([[r, 1, keys - 1, r * nb, nb] for r in range(rows)], dtype=torch.int32, device="cuda")
     q = torch.randn(rows, qh, d, device="cuda").bfloat16()
+    if args.quantized:
+        cache = _quantized(cache)
     us = _time(lambda: ops.paged_decode(q, cache, table, seg, kvh, keys, keys_per_split=args.split,
                                         warps=args.warps, stages=args.stages),
                args.warmup, args.iters)
-    kv_bytes = rows * keys * kvh * d * 2 * 2
-    return dict(kernel="paged_decode", rows=rows, keys=keys, kv_heads=kvh, split=args.split, us=round(us, 2),
+    kv_bytes = rows * keys * kvh * 2 * (d + 4 if args.quantized else 2 * d)
+    return dict(kernel="paged_decode", quantized=args.quantized, rows=rows, keys=keys, kv_heads=kvh, split=args.split, us=round(us, 2),
                 kv_gbs=round(kv_bytes / us / 1e3, 1))
+
+
+def _quantized(cache):
+    """BF16 pages [blocks, 2, heads, 16, d] as a QuantizedCache."""
+    from furiosa_opt_models_b200 import ops
+
+    out = ops.QuantizedCache.empty(cache.shape[0], cache.shape[2], cache.shape[4])
+    scales = cache.float().abs().amax(-1).clamp_min_(1e-10) / 448
+    out.codes.view(torch.float8_e4m3fn).copy_((cache.float() / scales[..., None]).clamp_(-448, 448).to(torch.float8_e4m3fn))
+    out.scales.copy_(scales)
+    return out
+
+
+def tree_attn(args) -> dict:
+    from furiosa_opt_models_b200 import ops
+
+    n, nodes, cached, qh, kvh, d = args.trees, args.nodes, args.keys, args.q_heads, args.kv_heads, 128
+    nb = (cached + nodes + 15) // 16
+    cache = torch.randn(n * nb, 2, kvh, 16, d, device="cuda").bfloat16()
+    if args.quantized:
+        cache = _quantized(cache)
+    table = torch.randperm(n * nb, device="cuda").int()
+    seg = torch.tensor([[i * nodes, nodes, cached, i * nb, nb] for i in range(n)], dtype=torch.int32, device="cuda")
+    mask = ops.tree_mask([[-1] + [(i - 1) // 2 for i in range(1, nodes)]] * n).cuda()
+    q = torch.randn(n * nodes, qh, d, device="cuda").bfloat16()
+    us = _time(lambda: ops.paged_tree(q, cache, table, seg, kvh, cached + nodes, nodes, mask=mask), args.warmup, args.iters)
+    kv_bytes = n * (cached + nodes) * kvh * 2 * (d + 4 if args.quantized else 2 * d)
+    flops = 4 * n * nodes * (cached + nodes) * qh * d
+    return dict(kernel="paged_tree", trees=n, nodes=nodes, keys=cached, quantized=args.quantized, us=round(us, 2),
+                kv_gbs=round(kv_bytes / us / 1e3, 1), tflops=round(flops / us / 1e6, 1))
+
+
+def kv_store(args) -> dict:
+    from furiosa_opt_models_b200 import ops
+
+    rows, qh, kvh, d = args.rows, args.q_heads, args.kv_heads, 128
+    qkv = torch.randn(rows, (qh + 2 * kvh) * d, device="cuda").bfloat16()
+    cache = ops.QuantizedCache.empty((rows + 15) // 16, kvh, d)
+    at = torch.arange(rows, dtype=torch.int32, device="cuda")
+    norm = torch.ones(d, device="cuda").bfloat16()
+    freq = 1e6 ** (-torch.arange(0, d, 2, device="cuda").float() / d)
+    us = _time(lambda: ops.qk_norm_rope_cache(qkv, qh, kvh, d, norm, norm, 1e-6, at, freq, 1.0, cache, at),
+               args.warmup, args.iters)
+    moved = rows * ((qh + 2 * kvh) * d * 2 + qh * d * 2 + 2 * kvh * (d + 4) + 8)
+    return dict(kernel="kv_store", rows=rows, q_heads=qh, kv_heads=kvh, us=round(us, 2), gbs=round(moved / us / 1e3, 1))
+
+
+def logits(args) -> dict:
+    from furiosa_opt_models_b200 import ops
+
+    rows, vocab = args.rows, args.vocab
+    x = torch.randn(rows, vocab, device="cuda")
+    x = x.bfloat16() if args.half else x
+    out = torch.empty_like(x) if args.write else None
+    starts = torch.arange(rows + 1, dtype=torch.int32, device="cuda") * args.tokens
+    tokens = torch.randint(0, vocab, (rows * args.tokens,), dtype=torch.int32, device="cuda")
+    some = torch.full((rows,), 0.5, device="cuda")
+    us = _time(lambda: ops.process_logits(x, output=(tokens, starts), frequency=some, presence=some, out=out),
+               args.warmup, args.iters)
+    moved = x.numel() * x.element_size() * (2 if args.write else 1)
+    return dict(kernel="process_logits", rows=rows, vocab=vocab, tokens=args.tokens, us=round(us, 2),
+                gbs=round(moved / us / 1e3, 1))
 
 
 def prefill_attn(args) -> dict:
@@ -280,6 +344,24 @@ def main() -> None:
     d.add_argument("--split", type=int, default=2048, help="keys per split")
     d.add_argument("--warps", type=int, default=0, help="warps a CTA (2-4; 0 the engine's default)")
     d.add_argument("--stages", type=int, default=0, help="16-key blocks in flight a warp (2-3; 0 default)")
+    d.add_argument("--quantized", action="store_true", help="E4M3 pages instead of BF16 ones")
+    t = sub.add_parser("tree-attn")
+    t.add_argument("--trees", type=int, default=16)
+    t.add_argument("--nodes", type=int, default=64)
+    t.add_argument("--keys", type=int, default=8192)
+    t.add_argument("--q-heads", type=int, default=32)
+    t.add_argument("--kv-heads", type=int, default=8)
+    t.add_argument("--quantized", action="store_true", help="E4M3 pages instead of BF16 ones")
+    k = sub.add_parser("kv-store")
+    k.add_argument("--rows", type=int, default=8192)
+    k.add_argument("--q-heads", type=int, default=32)
+    k.add_argument("--kv-heads", type=int, default=8)
+    lg = sub.add_parser("logits")
+    lg.add_argument("--rows", type=int, default=64)
+    lg.add_argument("--vocab", type=int, default=151936)
+    lg.add_argument("--tokens", type=int, default=512, help="output tokens of a row")
+    lg.add_argument("--half", action="store_true", help="BF16 logits")
+    lg.add_argument("--write", action="store_true", help="write the adjusted logits")
     f = sub.add_parser("prefill-attn")
     f.add_argument("--rows", type=int, default=8192)
     f.add_argument("--seqs", type=int, default=8)
@@ -291,12 +373,12 @@ def main() -> None:
     a = sub.add_parser("tp-o-proj")
     a.add_argument("--rows", type=int, default=64)
     a.add_argument("--model", default="qwen3-1.7b")
-    for s in (g, d, f, m, a):
+    for s in (g, d, t, k, lg, f, m, a):
         s.add_argument("--warmup", type=int, default=3)
         s.add_argument("--iters", type=int, default=10)
     args = p.parse_args()
     out = {"gemm": gemm, "decode-attn": decode_attn, "prefill-attn": prefill_attn, "moe": moe,
-           "tp-o-proj": tp_o_proj}[args.what](args)
+           "tree-attn": tree_attn, "kv-store": kv_store, "logits": logits, "tp-o-proj": tp_o_proj}[args.what](args)
     if out.pop("_rank", 0) == 0:
         print(json.dumps(out), flush=True)
 
