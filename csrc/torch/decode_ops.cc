@@ -3,6 +3,7 @@
 // first tensor's device and that device's current stream. Decode calls are short, and in Python the
 // checks alone took 8 of a call's 16 us. This module is built against torch; the kernels stay in the
 // engine's extension (which needs no torch) and are called through the addresses it gives out.
+#include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -283,6 +284,17 @@ py::object tree_attention(py::handle q, py::handle cache, int quantized_dim, py:
   return o;
 }
 
+// Views of quantized pages (checked by their class): the rows' codes, and their scales.
+py::object codes(py::handle pages, long d) {
+  const at::Tensor& x = THPVariable_Unpack(pages.ptr());
+  const int64_t page = x.size(3), heads = x.size(2) * page;
+  return wrap(x.as_strided({x.size(0), 2, x.size(2), 16, d}, {2 * heads, heads, page, d, 1}));
+}
+py::object scales(py::handle pages, long d) {
+  const at::Tensor& x = THPVariable_Unpack(pages.ptr());
+  return wrap(x.slice(3, 16 * d).view(at::kFloat));
+}
+
 // (tokens, ..., starts): row r's tokens are tokens[starts[r] .. starts[r + 1]).
 foa::TokenLists token_lists(py::handle lists, long rows, const char* name, const Place& place) {
   foa::TokenLists l;
@@ -395,6 +407,8 @@ PYBIND11_MODULE(_calls, m) {
     run.process_logits = reinterpret_cast<decltype(run.process_logits)>(process_logits);
     run.logits_slices = reinterpret_cast<decltype(run.logits_slices)>(logits_slices);
   });
+  m.def("codes", &codes);
+  m.def("scales", &scales);
   m.def("kv_store", &kv_store);
   m.def("tree_attention", &tree_attention);
   m.def("process_logits", &process_logits);

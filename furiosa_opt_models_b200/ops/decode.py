@@ -63,14 +63,12 @@ class QuantizedCache:
     @property
     def codes(self) -> torch.Tensor:
         """The E4M3 codes as a uint8 view [blocks, 2, kv_heads, 16, head_dim]."""
-        p, d = self.pages, self.head_dim
-        blocks, _, heads, page = p.shape
-        return p.as_strided((blocks, 2, heads, BLOCK, d), (2 * heads * page, heads * page, page, d, 1))
+        return calls().codes(self.pages, self.head_dim)
 
     @property
     def scales(self) -> torch.Tensor:
         """The scales as an FP32 view [blocks, 2, kv_heads, 16]."""
-        return self.pages[..., BLOCK * self.head_dim:].view(torch.float32)
+        return calls().scales(self.pages, self.head_dim)
 
     def dequantize(self) -> torch.Tensor:
         """The values the cache stands for, FP32 [blocks, 2, kv_heads, 16, head_dim]."""
