@@ -704,12 +704,15 @@ int launch(const TreeAttention& p, cudaStream_t stream) {
   return merge<D>(p, splits, stream);
 }
 
-// Whether a segment may have more rows than the mma.sync form holds in one tile.
-bool tc_rows(int max_len, int group) { return (long)max_len * group > 16; }
+// Whether a segment may have more rows than the mma.sync form holds in one tile, or in two over codes,
+// where a second pass over the pages (from L2) costs less than a tcgen05 tile that is a quarter full:
+// 64 trees of 5 nodes, 4 heads a key/value head, up to 4096 keys: 116 us in two tiles, 175 by tcgen05;
+// 16 of 8 nodes, up to 8192 keys: 80 and 95. (BF16: 89 and 85.)
+bool tc_rows(int max_len, int group, bool quantized) { return (long)max_len * group > (quantized ? 32 : 16); }
 
 template <int D, bool kQ>
 int pick(const TreeAttention& p, cudaStream_t stream) {
-  if (tc_rows(p.max_len, p.q_heads / p.kv_heads) && tree_attention_tc_supported(p)) {
+  if (tc_rows(p.max_len, p.q_heads / p.kv_heads, kQ) && tree_attention_tc_supported(p)) {
     const int rc = tree_attention_tc(p, stream);
     return rc != 0 ? rc : merge<D>(p, (p.max_keys + p.keys_per_split - 1) / p.keys_per_split, stream);
   }
@@ -722,15 +725,20 @@ int tree_attention_split(int num_segments, int q_heads, int kv_heads, int head_d
                          int max_len) {
   if (num_segments <= 0 || kv_heads <= 0 || max_keys <= 0) return 16;
   const long rows = (long)max_len * (q_heads / kv_heads);
-  const bool tc = tc_rows(max_len, (int)(q_heads / kv_heads));
+  const bool tc = tc_rows(max_len, (int)(q_heads / kv_heads), quantized != 0);
   const long tile = tc ? 256 : 16;
   const long items = (rows + tile - 1) / tile * kv_heads * num_segments;
   // About two (tcgen05) or three CTAs for each that the GPU holds at once (segments may differ in
   // length), of at least so many keys that a CTA's start and end do not count; fewer where the GPU is
   // far from full (one sequence of 1000 keys, 8 heads: 8.2 us in splits of 128, 9.5 of 256; four of
-  // 2048: 11.4 and 10.8).
-  const long want = tc ? 148L * 2 : 148L * 16;
-  const long least = tc ? 512 : items * (((long)max_keys + 127) / 128) <= 148L * 2 ? 128 : 256;
+  // 2048: 11.4 and 10.8). Long histories are cut into 96 parts at most, since each is joined again, and
+  // where a key/value head has more than 8 rows, each part of which leaves as much as 60 keys take,
+  // into 32 (one of 32768 keys, 16 rows: 26 us in splits of 1024, 39 of 256).
+  const bool wide = !tc && rows > 8;
+  const long want = tc ? 148L * 2 : wide ? 148L * 9 : 148L * 16;
+  const long parts = tc ? max_keys : wide ? 32 : 96;
+  const long thin = items * (((long)max_keys + 127) / 128) <= 148L * 2 ? 128 : 256;
+  const long least = tc ? 512 : (max_keys + parts - 1) / parts > thin ? (max_keys + parts - 1) / parts : thin;
   const long per = ((long)max_keys * items + want - 1) / want;
   const long keys = ((per < least ? least : per) + 127) / 128 * 128;
   return (int)(keys > max_keys ? (max_keys + 15) / 16 * 16 : keys);
