@@ -349,26 +349,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
       const uint32_t dst = smem_u32(smem + C::kOffQ + (two ? w : 0) * C::kQTile);
       const bool store = two || w == 0;
+      uint4 raw[D / 8];  // the whole row, in one trip to L2
+#pragma unroll
+      for (int ch = 0; ch < D / 8; ++ch) raw[ch] = real ? reinterpret_cast<const uint4*>(src)[ch] : make_uint4(0u, 0u, 0u, 0u);
       if constexpr (kQ) {
         float amax = 0.f;
-        if (real)
-#pragma unroll 4
-          for (int ch = 0; ch < D / 8; ++ch) {
-            const uint4 v = reinterpret_cast<const uint4*>(src)[ch];
-            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(bf16_lo(v.x)), fabsf(bf16_hi(v.x))), fmaxf(fabsf(bf16_lo(v.y)), fabsf(bf16_hi(v.y)))));
-            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(bf16_lo(v.z)), fabsf(bf16_hi(v.z))), fmaxf(fabsf(bf16_lo(v.w)), fabsf(bf16_hi(v.w)))));
-          }
+#pragma unroll
+        for (int ch = 0; ch < D / 8; ++ch) {
+          const uint4 v = raw[ch];
+          amax = fmaxf(amax, fmaxf(fmaxf(fabsf(bf16_lo(v.x)), fabsf(bf16_hi(v.x))), fmaxf(fabsf(bf16_lo(v.y)), fabsf(bf16_hi(v.y)))));
+          amax = fmaxf(amax, fmaxf(fmaxf(fabsf(bf16_lo(v.z)), fabsf(bf16_hi(v.z))), fmaxf(fabsf(bf16_lo(v.w)), fabsf(bf16_hi(v.w)))));
+        }
         const int e = min(max((int)(__float_as_uint(amax) >> 23), 8), 254) - 127;
         const float down = __uint_as_float((uint32_t)(127 + 7 - e) << 23);  // 7 - e in [-120, 126]
         c = fmaxf(c * __uint_as_float((uint32_t)(127 - 7 + e) << 23), 1.2e-38f);
         if (store)
-#pragma unroll 2
+#pragma unroll
           for (int ch = 0; ch < D / 16; ++ch) {
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              uint4 v = make_uint4(0u, 0u, 0u, 0u);
-              if (real) v = reinterpret_cast<const uint4*>(src)[2 * ch + half];
+              const uint4 v = raw[2 * ch + half];
               const uint32_t vw[4] = {v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip};
               uint16_t h[4], l[4];
 #pragma unroll
@@ -390,10 +391,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             sts128(dst + C::kTile8 + at8<D>(row, ch), make_uint4(lo[0], lo[1], lo[2], lo[3]));
           }
       } else if (store) {
-#pragma unroll 4
+#pragma unroll
         for (int ch = 0; ch < D / 8; ++ch) {
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (real) v = reinterpret_cast<const uint4*>(src)[ch];
+          const uint4 v = raw[ch];
           sts128(dst + at16(row, ch), make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip));
         }
       }
