@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int32_t* table = p.table + seg.table_start;
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, two ? 256 : 128);
+    mbar_init(q_full, 256);
     for (int s = 0; s < 3; ++s) {
       mbar_init(k_full + s, 1);
       mbar_init(k_empty + s, 1);
@@ -342,65 +342,66 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int tok = real ? m / G : 0, head = kvh * G + (real ? m % G : 0);
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_col = lane_base + w * kTile, o_col = lane_base + C::kColO + w * kTile;
-    // Q: this row into the tile (by the first warpgroup alone where both share it).
+    // Q: this row into its tile (half of its columns where both warpgroups share the tile).
     float c = fmaxf(fabsf(p.scale) * kLog2e, 1.2e-38f);  // (a negative scale turns q's sign)
     {
       const __nv_bfloat16* src = p.q + (long)(seg.row_start + tok) * p.ld_q + (long)head * D;
       const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
       const uint32_t dst = smem_u32(smem + C::kOffQ + (two ? w : 0) * C::kQTile);
-      const bool store = two || w == 0;
+      // Chunk x of n is this warpgroup's.
+      auto mine = [&](int x, int n) { return two || (x >= n / 2) == (w == 1); };
       uint4 raw[D / 8];  // the whole row, in one trip to L2
 #pragma unroll
       for (int ch = 0; ch < D / 8; ++ch) raw[ch] = real ? reinterpret_cast<const uint4*>(src)[ch] : make_uint4(0u, 0u, 0u, 0u);
       if constexpr (kQ) {
-        float amax = 0.f;
+        // The largest magnitude, as BF16 bits.
+        uint32_t most = 0u;
 #pragma unroll
         for (int ch = 0; ch < D / 8; ++ch) {
           const uint4 v = raw[ch];
-          amax = fmaxf(amax, fmaxf(fmaxf(fabsf(bf16_lo(v.x)), fabsf(bf16_hi(v.x))), fmaxf(fabsf(bf16_lo(v.y)), fabsf(bf16_hi(v.y)))));
-          amax = fmaxf(amax, fmaxf(fmaxf(fabsf(bf16_lo(v.z)), fabsf(bf16_hi(v.z))), fmaxf(fabsf(bf16_lo(v.w)), fabsf(bf16_hi(v.w)))));
+          most = __vmaxu2(most, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
         }
-        const int e = min(max((int)(__float_as_uint(amax) >> 23), 8), 254) - 127;
-        const float down = __uint_as_float((uint32_t)(127 + 7 - e) << 23);  // 7 - e in [-120, 126]
+        most = max(most >> 16, most & 0xffffu);
+        const int e = min(max((int)(most >> 7), 8), 254) - 127;
+        // 7 - e in [-120, 126]. A row with an element that is not finite has no finite score: it is NaN
+        // throughout (the conversion would saturate it).
+        const float down = most >= 0x7f80u ? __int_as_float(0x7fffffff) : __uint_as_float((uint32_t)(127 + 7 - e) << 23);
         c = fmaxf(c * __uint_as_float((uint32_t)(127 - 7 + e) << 23), 1.2e-38f);
-        if (store)
 #pragma unroll
-          for (int ch = 0; ch < D / 16; ++ch) {
-            uint32_t hi[4], lo[4];
+        for (int ch = 0; ch < D / 16; ++ch) {
+          if (!mine(ch, D / 16)) continue;
+          uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const uint4 v = raw[2 * ch + half];
-              const uint32_t vw[4] = {v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip};
-              uint16_t h[4], l[4];
+          for (int half = 0; half < 2; ++half) {
+            const uint4 v = raw[2 * ch + half];
+            const uint32_t vw[4] = {v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip};
+            uint16_t h[4], l[4];
 #pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                float2 f = make_float2(bf16_lo(vw[x]) * down, bf16_hi(vw[x]) * down);
-                if (!(fabsf(f.x) < INFINITY)) f.x = __int_as_float(0x7fffffff);  // (the conversion saturates)
-                if (!(fabsf(f.y) < INFINITY)) f.y = __int_as_float(0x7fffffff);
-                h[x] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
-                const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2(h[x], __NV_E4M3);
-                const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&hr));
-                l[x] = __nv_cvt_float2_to_fp8x2(make_float2(f.x - hf.x, f.y - hf.y), __NV_SATFINITE, __NV_E4M3);
-              }
-              hi[2 * half] = h[0] | (uint32_t)h[1] << 16;
-              hi[2 * half + 1] = h[2] | (uint32_t)h[3] << 16;
-              lo[2 * half] = l[0] | (uint32_t)l[1] << 16;
-              lo[2 * half + 1] = l[2] | (uint32_t)l[3] << 16;
+            for (int x = 0; x < 4; ++x) {
+              const float2 f = make_float2(bf16_lo(vw[x]) * down, bf16_hi(vw[x]) * down);
+              h[x] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+              const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2(h[x], __NV_E4M3);
+              const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&hr));
+              l[x] = __nv_cvt_float2_to_fp8x2(make_float2(f.x - hf.x, f.y - hf.y), __NV_SATFINITE, __NV_E4M3);
             }
-            sts128(dst + at8<D>(row, ch), make_uint4(hi[0], hi[1], hi[2], hi[3]));
-            sts128(dst + C::kTile8 + at8<D>(row, ch), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+            hi[2 * half] = h[0] | (uint32_t)h[1] << 16;
+            hi[2 * half + 1] = h[2] | (uint32_t)h[3] << 16;
+            lo[2 * half] = l[0] | (uint32_t)l[1] << 16;
+            lo[2 * half + 1] = l[2] | (uint32_t)l[3] << 16;
           }
-      } else if (store) {
+          sts128(dst + at8<D>(row, ch), make_uint4(hi[0], hi[1], hi[2], hi[3]));
+          sts128(dst + C::kTile8 + at8<D>(row, ch), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+        }
+      } else {
 #pragma unroll
         for (int ch = 0; ch < D / 8; ++ch) {
+          if (!mine(ch, D / 8)) continue;
           const uint4 v = raw[ch];
           sts128(dst + at16(row, ch), make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip));
         }
       }
-      if (store) {
-        fence_proxy_async();
-        mbar_arrive(q_full);
-      }
+      fence_proxy_async();
+      mbar_arrive(q_full);
     }
     const bool idle = !__any_sync(0xffffffffu, real);  // none of the warp's rows counts
     float top = -INFINITY, sum = 0.f;
@@ -536,6 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // (B) The second warpgroup's sums go through the key and value stages, free by now.
     float* other = reinterpret_cast<float*>(smem + C::kOffK);
     static_assert(kTile * D * 4 <= C::kOffScale - C::kOffK, "the join fits the stages");
+    static_assert(8 * 4096 <= C::kOffK - C::kOffQ, "the warps' boxes fit Q's tiles");
     auto other_at = [&](int ch) { return other + row * D + ((ch ^ row) & (D / 4 - 1)) * 4; };  // 4 columns
     if (!two && w == 1) {
       if (fine) {
@@ -617,10 +619,22 @@ __global__ void __launch_bounds__(kThreads, 1)
               *reinterpret_cast<uint4*>(dst + c0 + x) =
                   make_uint4(pack_bf16x2(v[x] * norm, v[x + 1] * norm), pack_bf16x2(v[x + 2] * norm, v[x + 3] * norm),
                              pack_bf16x2(v[x + 4] * norm, v[x + 5] * norm), pack_bf16x2(v[x + 6] * norm, v[x + 7] * norm));
-          } else if (real) {
+          } else if (nsplit > 1) {
+            // Through Q's tile, free by now, so that eight lanes write a row's 128 bytes.
+            const uint32_t box = smem_u32(smem + C::kOffQ) + warp * 4096;
 #pragma unroll
-            for (int x = 0; x < 32; x += 4)
-              *reinterpret_cast<float4*>(part + c0 + x) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+            for (int x = 0; x < 8; ++x)
+              sts128(box + lane * 128 + ((x ^ lane & 7) << 4),
+                     make_uint4(__float_as_uint(v[4 * x]), __float_as_uint(v[4 * x + 1]), __float_as_uint(v[4 * x + 2]),
+                                __float_as_uint(v[4 * x + 3])));
+            __syncwarp();
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              const int r1 = 4 * x + (lane >> 3);
+              float* to = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, real ? reinterpret_cast<uint64_t>(part) : 0ull, r1));
+              const uint4 y = lds128(box + r1 * 128 + (((lane & 7) ^ (r1 & 7)) << 4));
+              if (to != nullptr) *reinterpret_cast<uint4*>(to + c0 + 4 * (lane & 7)) = y;
+            }
           }
         }
         if (real && nsplit > 1) p.partial_ml[idx] = make_float2(top, sum);
