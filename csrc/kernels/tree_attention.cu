@@ -35,6 +35,7 @@
 #include "decode_ops.cuh"
 #include "launch.cuh"
 #include "sm100.cuh"
+#include "tree_split.cuh"
 
 namespace foa {
 namespace {
@@ -204,10 +205,11 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
   const int M = seg.len * G;
   const int m0 = mt * kRows;
   const int keys = seg.cached + seg.len;
-  const int nsplit = (keys + p.keys_per_split - 1) / p.keys_per_split;
+  const Parts parts(keys, p.keys_per_split, false);
+  const int nsplit = parts.count;
   if (m0 >= M || split >= nsplit) return;
-  const int k0 = split * p.keys_per_split;
-  const int k1 = min(keys, k0 + p.keys_per_split);
+  const int k0 = split * parts.width;
+  const int k1 = min(keys, k0 + parts.width);
 
   const uint32_t wbase = smem_u32(smem) + warp * kStages * 2 * P::kSlot;
   const uint8_t* cache = static_cast<const uint8_t*>(p.cache);
@@ -614,7 +616,7 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
 // keys and 16 heads in 256 splits took 77 us, with sixteen 60. How many take part follows from the
 // row's own splits, so that the order of its sums is the same in every call.
 template <int D, int W>
-__global__ void __launch_bounds__(32 * W) tree_merge_kernel(const TreeAttention p, int max_splits) {
+__global__ void __launch_bounds__(32 * W) tree_merge_kernel(const TreeAttention p, int max_splits, bool even) {
   constexpr int E = D / 32;
   __shared__ float sm_acc[W - 1][D], sm_den[W - 1];
   pdl_wait();
@@ -623,7 +625,7 @@ __global__ void __launch_bounds__(32 * W) tree_merge_kernel(const TreeAttention 
   const int tok = blockIdx.x % p.max_len;
   const int head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (tok >= seg.len || !rows_fit(p, seg) || !segment_fits(p, seg)) return;
-  const int nsplit = (seg.cached + seg.len + p.keys_per_split - 1) / p.keys_per_split;
+  const int nsplit = Parts(seg.cached + seg.len, p.keys_per_split, even).count;
   if (nsplit == 1) return;  // written in place
   const int warps = nsplit > 16 ? 16 : 4;  // (the launch has sixteen when a row may need them)
   const long row = seg.row_start + tok;
@@ -675,11 +677,11 @@ __global__ void __launch_bounds__(32 * W) tree_merge_kernel(const TreeAttention 
 }
 
 template <int D>
-int merge(const TreeAttention& p, int splits, cudaStream_t stream) {
+int merge(const TreeAttention& p, int splits, bool even, cudaStream_t stream) {
   if (splits == 1) return 0;
   const dim3 grid(p.num_segments * p.max_len, p.q_heads);
-  const cudaError_t rc = splits > 16 ? launch_pdl(tree_merge_kernel<D, 16>, grid, dim3(512), 0, stream, p, splits)
-                                     : launch_pdl(tree_merge_kernel<D, 4>, grid, dim3(128), 0, stream, p, splits);
+  const cudaError_t rc = splits > 16 ? launch_pdl(tree_merge_kernel<D, 16>, grid, dim3(512), 0, stream, p, splits, even)
+                                     : launch_pdl(tree_merge_kernel<D, 4>, grid, dim3(128), 0, stream, p, splits, even);
   return rc == cudaSuccess ? 0 : -5;
 }
 
@@ -701,7 +703,7 @@ int launch(const TreeAttention& p, cudaStream_t stream) {
   }
   if (launch_pdl(kernel, dim3((unsigned)ctas, splits), dim3(32 * kWarps), smem, stream, p, (int)mtiles, splits) != cudaSuccess)
     return -5;
-  return merge<D>(p, splits, stream);
+  return merge<D>(p, splits, false, stream);
 }
 
 // Whether a segment may have more rows than the mma.sync form holds in one tile, or in two over codes,
@@ -714,7 +716,7 @@ template <int D, bool kQ>
 int pick(const TreeAttention& p, cudaStream_t stream) {
   if (tc_rows(p.max_len, p.q_heads / p.kv_heads, kQ) && tree_attention_tc_supported(p)) {
     const int rc = tree_attention_tc(p, stream);
-    return rc != 0 ? rc : merge<D>(p, (p.max_keys + p.keys_per_split - 1) / p.keys_per_split, stream);
+    return rc != 0 ? rc : merge<D>(p, (p.max_keys + p.keys_per_split - 1) / p.keys_per_split, true, stream);
   }
   return (long)p.max_len * (p.q_heads / p.kv_heads) <= 8 ? launch<D, kQ, 1>(p, stream) : launch<D, kQ, 2>(p, stream);
 }

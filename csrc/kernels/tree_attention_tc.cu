@@ -27,7 +27,9 @@
 // overwrites P), overlapped with the other one's; over codes the shared-memory pipe beside it, since
 // every thread reads every key's two scales (a broadcast of 16 bytes takes as long as 512 bytes) while
 // the MMAs read Q, K and V there. 24 trees of 32 to 64 nodes over 4.5 to 16.4 thousand keys, 32 x 8
-// heads of 128: 460 us over codes, 335 over BF16 pages (590 TFLOP/s); 16 of 16 to 31 nodes: 127 and 120.
+// heads of 128: 432 us over codes, 326 over BF16 pages (604 TFLOP/s); 16 of 16 to 31 nodes: 117 and 112. A CTA holds its SM alone, so its start and
+// end (5 and 6 us before both warpgroups converted Q and rows were written 128 bytes at a time) and
+// unequal parts show in full: 462 and 128 us with parts cut every keys_per_split keys.
 // An mbarrier wait costs the MMA thread 200 cycles even for a phase long complete, so what is surely
 // there (K, V, scales) is waited for before what is not (P, S): 496 -> 462 us. Tried and slower, over
 // the same trees with the kernel of that day: S in halves of 64 keys so that S overlaps the softmax
@@ -42,6 +44,7 @@
 #include "launch.cuh"
 #include "sm100.cuh"
 #include "tmap.cuh"
+#include "tree_split.cuh"
 
 namespace foa {
 namespace {
@@ -292,10 +295,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int M = seg.len * G;
   const int m0 = mt * 2 * kTile;
   const int keys = seg.cached + seg.len;
-  const int nsplit = (keys + p.keys_per_split - 1) / p.keys_per_split;
+  const Parts parts(keys, p.keys_per_split, true);
+  const int nsplit = parts.count;
   if (m0 >= M || split >= nsplit) return;
-  const int k0 = split * p.keys_per_split;
-  const int k1 = min(keys, k0 + p.keys_per_split);
+  const int k0 = split * parts.width;
+  const int k1 = min(keys, k0 + parts.width);
   const int ntiles = (k1 - k0 + kTile - 1) / kTile;
   const bool two = M - m0 > kTile;          // (A) two row tiles
   const int steps = two ? 2 * ntiles : ntiles;  // (warpgroup, key tile) pairs in turn

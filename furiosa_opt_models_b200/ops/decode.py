@@ -116,8 +116,8 @@ def paged_tree(q, cache, table, segments, kv_heads, max_keys, max_len, mask=None
 
     ``max_keys`` bounds every segment's cached + len and ``max_len`` its len: a segment that goes
     past one of them (or past its table or the rows) gets zeros and records a status. A history is
-    split every ``keys_per_split`` keys (a multiple of 16), and the splits are joined in order; by
-    default the width depends on the sizes of the call, so a fixed width is what keeps a row's bits
+    split into parts of at most ``keys_per_split`` keys (a multiple of 16), which are joined in order;
+    by default the width depends on the sizes of the call, so a fixed width is what keeps a row's bits
     the same in other batches (of the same ``max_len``, which picks the kernel)."""
     quantized = isinstance(cache, QuantizedCache)
     return calls().tree_attention(q, cache.pages if quantized else cache, cache.head_dim if quantized else 0, table,

@@ -463,6 +463,25 @@ def test_a_fixed_split_gives_the_same_bits_in_any_batch():
     assert torch.equal(whole[3], one[3])
 
 
+@pytest.mark.parametrize("quantized", [True, False], ids=["e4m3", "bf16"])
+@pytest.mark.parametrize("n", [20, 40])
+def test_parts_of_histories_around_whole_tiles(n, quantized):
+    """Histories that end on, before and behind a tile, in parts of one to five tiles."""
+    ops = _ops()
+    gen = torch.Generator().manual_seed(n)
+    hq, hk, d = 8, 2, 128
+    cached = [0, 127 - n, 128 - n, 129 - n, 255, 256 - n, 257, 640 - n, 641 - n, 900]
+    lens = [n] * len(cached)
+    cache, table, segs, values, tab, sl = _paged(lens, cached, hk, d, quantized, gen)
+    masks = _random_masks(lens, gen)
+    q = torch.randn(sum(lens), hq, d, generator=gen).to(BF16)
+    ref, weight, err = _attend64(q, values, tab, sl, d ** -0.5, mask=masks)
+    for split in (128, 256, 384, 640):
+        out = ops.paged_tree(q.to(DEV), cache, table, segs, hk, max(cached) + n, n, mask=_pack(masks), keys_per_split=split)
+        _check()
+        assert ((out.double().cpu() - ref).abs() <= _tolerance(ref, weight, err, d, quantized)).all()
+
+
 def test_a_long_row_of_many_splits_has_the_same_bits_in_any_batch():
     ops = _ops()
     gen = torch.Generator().manual_seed(8)
