@@ -179,8 +179,8 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
 
 // Bounded waits of one thread and of a whole warp, in few instructions (sm100's with its clock, at
 // twenty places beside five roles' code, pushed the softmax loop out of the instruction cache). A
-// poll blocks for some time by itself; the limit is on their number.
-constexpr uint32_t kPolls = 1u << 22;
+// poll blocks for 1.4 us by itself, so the limit on their number is one of 3 s.
+constexpr uint32_t kPolls = 1u << 21;
 __device__ __forceinline__ bool gave_up(uint32_t polls, int* status, int site, volatile int* abort) {
   if (polls & 63u) return false;
   if (abort != nullptr && *abort) return true;
