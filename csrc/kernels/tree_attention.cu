@@ -108,10 +108,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-}
 // Transposes the warp's 8 x 8 matrix of 16-bit values (row g, columns 2t and 2t + 1 a lane).
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t r;
@@ -275,17 +271,20 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
       const int e = kQ ? 16 * (t + 4 * (s >> 2)) + 4 * (s & 3) : 8 * (t + 4 * (s >> 1)) + 4 * (s & 1);
       raw[s] = src != nullptr ? *reinterpret_cast<const uint2*>(src + e) : make_uint2(0u, 0u);
     }
-    float c = p.scale * kLog2e;
-    if constexpr (kQ) {
-      float amax = 0.f;
+    // The row's largest magnitude, as BF16 bits.
+    uint32_t most = 0u;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-        amax = fmaxf(amax, fmaxf(fmaxf(fabsf(bf16_lo(raw[s].x)), fabsf(bf16_hi(raw[s].x))),
-                                 fmaxf(fabsf(bf16_lo(raw[s].y)), fabsf(bf16_hi(raw[s].y)))));
-      amax = quad_max(amax);
-      // 2^e <= amax < 2^(e+1): q * 2^(14 - e) stays below FP16's 65504 and loses only what lies
+    for (int s = 0; s < kSteps; ++s) most = __vmaxu2(most, __vmaxu2(raw[s].x & 0x7fff7fffu, raw[s].y & 0x7fff7fffu));
+    most = max(most >> 16, most & 0xffffu);
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    // A row with an element that is not finite has no finite score: what it sees makes it NaN (of an
+    // infinity's products those of one sign would pass for keys that are not seen).
+    float c = most >= 0x7f80u ? __int_as_float(0x7fffffff) : p.scale * kLog2e;
+    if constexpr (kQ) {
+      // 2^e <= the largest < 2^(e+1): q * 2^(14 - e) stays below FP16's 65504 and loses only what lies
       // 2^-38 below the row's largest.
-      const int e = min(max((int)(__float_as_uint(amax) >> 23), 15), 254) - 127;
+      const int e = min(max((int)(most >> 7), 15), 254) - 127;
       const float down = __uint_as_float((uint32_t)(127 + 14 - e) << 23);  // 14 - e in [-113, 126]
       c *= __uint_as_float((uint32_t)(127 - 14 + e) << 23);
 #pragma unroll
@@ -630,8 +629,15 @@ __global__ void __launch_bounds__(32 * W) tree_merge_kernel(const TreeAttention 
   const int warps = nsplit > 16 ? 16 : 4;  // (the launch has sixteen when a row may need them)
   const long row = seg.row_start + tok;
   const long base = (row * p.q_heads + head) * max_splits;
+  // A part whose scores are all NaN has the maximum of one that sees nothing, and a sum that is NaN.
   float top = -INFINITY;
-  for (int s = lane; s < nsplit; s += 32) top = fmaxf(top, p.partial_ml[base + s].x);
+  bool nan = false;
+  for (int s = lane; s < nsplit; s += 32) {
+    const float2 ml = p.partial_ml[base + s];
+    top = fmaxf(top, ml.x);
+    nan = nan || ml.y != ml.y;
+  }
+  nan = __any_sync(0xffffffffu, nan);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   float acc[E], den = 0.f;
@@ -671,7 +677,8 @@ __global__ void __launch_bounds__(32 * W) tree_merge_kernel(const TreeAttention 
     for (int e = 0; e < E; ++e) acc[e] += sm_acc[w][lane * E + e];
   }
   __nv_bfloat16* dst = p.o + row * p.ld_o + (long)head * D + lane * E;
-  const float inv = top > -INFINITY ? 1.f / den : 0.f;
+  if (nan) den = __int_as_float(0x7fffffff);
+  const float inv = top > -INFINITY || nan ? 1.f / den : 0.f;
 #pragma unroll
   for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
 }

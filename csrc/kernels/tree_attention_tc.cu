@@ -357,19 +357,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint4 raw[D / 8];  // the whole row, in one trip to L2
 #pragma unroll
       for (int ch = 0; ch < D / 8; ++ch) raw[ch] = real ? reinterpret_cast<const uint4*>(src)[ch] : make_uint4(0u, 0u, 0u, 0u);
-      if constexpr (kQ) {
-        // The largest magnitude, as BF16 bits.
-        uint32_t most = 0u;
+      // The largest magnitude, as BF16 bits.
+      uint32_t most = 0u;
 #pragma unroll
-        for (int ch = 0; ch < D / 8; ++ch) {
-          const uint4 v = raw[ch];
-          most = __vmaxu2(most, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
-        }
-        most = max(most >> 16, most & 0xffffu);
+      for (int ch = 0; ch < D / 8; ++ch) {
+        const uint4 v = raw[ch];
+        most = __vmaxu2(most, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+      }
+      most = max(most >> 16, most & 0xffffu);
+      // A row with an element that is not finite has no finite score: it is NaN throughout (E4M3 would
+      // saturate an infinity, and of its products those of one sign would pass for keys that are not seen).
+      const bool finite = most < 0x7f80u;
+      if constexpr (kQ) {
         const int e = min(max((int)(most >> 7), 8), 254) - 127;
-        // 7 - e in [-120, 126]. A row with an element that is not finite has no finite score: it is NaN
-        // throughout (the conversion would saturate it).
-        const float down = most >= 0x7f80u ? __int_as_float(0x7fffffff) : __uint_as_float((uint32_t)(127 + 7 - e) << 23);
+        const float down = finite ? __uint_as_float((uint32_t)(127 + 7 - e) << 23) : __int_as_float(0x7fffffff);  // 7 - e in [-120, 126]
         c = fmaxf(c * __uint_as_float((uint32_t)(127 - 7 + e) << 23), 1.2e-38f);
 #pragma unroll
         for (int ch = 0; ch < D / 16; ++ch) {
@@ -401,7 +402,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int ch = 0; ch < D / 8; ++ch) {
           if (!mine(ch, D / 8)) continue;
           const uint4 v = raw[ch];
-          sts128(dst + at16(row, ch), make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip));
+          const uint32_t nan = finite ? 0u : 0x7fff7fffu;
+          sts128(dst + at16(row, ch), make_uint4(v.x ^ flip | nan, v.y ^ flip | nan, v.z ^ flip | nan, v.w ^ flip | nan));
         }
       }
       fence_proxy_async();
@@ -574,7 +576,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           top = both;
         }
         const bool fix = *reinterpret_cast<volatile int*>(odd_v) != 0;
-        const float norm = nsplit > 1 ? 1.f : top == -INFINITY ? 0.f : 1.f / sum;
+        // (Scores that are all NaN leave the maximum of a row that sees nothing, and a sum that is NaN.)
+        const float norm = nsplit > 1 ? 1.f : top == -INFINITY && sum == 0.f ? 0.f : 1.f / sum;
         const long at = (long)(seg.row_start + tok);
         const long idx = (at * p.q_heads + head) * max_splits + split;
         __nv_bfloat16* dst = p.o + at * p.ld_o + (long)head * D;

@@ -885,3 +885,55 @@ def test_a_first_call_is_not_captured(monkeypatch):
         y = x + 1  # noqa: F841
         with pytest.raises(RuntimeError, match="cannot be captured"):
             ops.process_logits(x)
+
+
+@pytest.mark.parametrize("quantized", [True, False], ids=["e4m3", "bf16"])
+@pytest.mark.parametrize("n", [1, 3, 6, 20, 70])
+def test_a_query_that_is_not_finite_gives_nan_in_any_split(n, quantized):
+    """Its row is NaN whether one part of the history answers it or several, zeros where it sees no
+    key; the other rows are as they would be."""
+    ops = _ops()
+    gen = torch.Generator().manual_seed(n)
+    hq, hk, d = 8, 2, 128
+    lens, cached = [n, n], [300, 0]
+    cache, table, segs, values, tab, sl = _paged(lens, cached, hk, d, quantized, gen)
+    ms = [torch.eye(n, dtype=torch.bool) for _ in lens]
+    q = torch.randn(2 * n, hq, d, generator=gen).to(BF16)
+    odd = q.clone()
+    odd[0, 1, 5], odd[n, 6, 7], odd[2 * n - 1, 0, 100] = float("nan"), float("inf"), -float("inf")
+    bad = torch.zeros(2 * n, hq, dtype=torch.bool)
+    bad[0, 1] = bad[n, 6] = bad[2 * n - 1, 0] = True
+    if n > 2:
+        ms[1][1] = False
+        odd[n + 1, 3, 0] = float("nan")
+    ref, weight, err = _attend64(q, values, tab, sl, d ** -0.5, mask=ms)
+    tol = _tolerance(ref, weight, err, d, quantized)
+    for split in (None, 16, 128, 4096):
+        out = ops.paged_tree(odd.to(DEV), cache, table, segs, hk, n + 300, n, mask=_pack(ms), keys_per_split=split).cpu()
+        _check()
+        assert out[bad].isnan().all(), split
+        assert ((out.double() - ref).abs() <= tol)[~bad].all(), split
+        if n > 2:
+            assert torch.count_nonzero(out[n + 1]) == 0
+
+
+@pytest.mark.parametrize("quantized", [True, False], ids=["e4m3", "bf16"])
+@pytest.mark.parametrize("n", [3, 20, 70])
+def test_a_row_whose_only_key_is_nan(n, quantized):
+    ops = _ops()
+    gen = torch.Generator().manual_seed(n)
+    hq, hk, d = 8, 2, 64
+    cache, table, segs, values, tab, sl = _paged([n], [0], hk, d, quantized, gen)
+    if quantized:
+        cache.pages[tab[0], 0, :, 2 * d + 9] = 0x7F  # node 2's key
+    else:
+        cache[tab[0], 0, :, 2, 9] = float("nan")
+    ms = [torch.eye(n, dtype=torch.bool)]
+    q = torch.randn(n, hq, d, generator=gen).to(BF16)
+    ref, weight, err = _attend64(q, values, tab, sl, d ** -0.5, mask=ms)
+    tol = _tolerance(ref, weight, err, d, quantized)
+    other = torch.arange(n) != 2
+    for split in (None, 16, 4096):
+        out = ops.paged_tree(q.to(DEV), cache, table, segs, hk, n, n, mask=_pack(ms), keys_per_split=split).cpu()
+        _check()
+        assert out[2].isnan().all() and ((out.double() - ref).abs() <= tol)[other].all()
