@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* joined = bars + 24;   // (B) the second warpgroup's sums are in shared memory
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* odd_v = reinterpret_cast<int*>(tmem_slot + 2);  // values that are not finite were left out
+  int* odd_v = reinterpret_cast<int*>(tmem_slot + 2);  // values or scales that are not finite were left out
   float* scales = reinterpret_cast<float*>(smem + C::kOffScale);
   int* exps = reinterpret_cast<int*>(scales + kSlots * 2 * kTile);
 
@@ -609,10 +609,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               const int key = seg.cached + a, id = table[key >> 4];
               if (id < 0 || id >= p.cache_blocks) continue;
               const uint8_t* vp = cache + ((long)id * 2 * p.kv_heads + p.kv_heads + kvh) * pb + (long)(key & 15) * D * (kQ ? 1 : 2);
+              // A value, or all of them by their scale: left out of the products, added where seen.
+              const float s = kQ ? *reinterpret_cast<const float*>(vp + (16 - (key & 15)) * D + (key & 15) * 4) : 1.f;
+              const bool all = !(fabsf(s) < INFINITY);
 #pragma unroll
               for (int x = 0; x < 32; ++x) {
                 if constexpr (kQ) {
-                  if ((vp[c0 + x] & 0x7fu) == 0x7fu) v[x] = __int_as_float(0x7fffffff);
+                  if (all || (vp[c0 + x] & 0x7fu) == 0x7fu)
+                    v[x] += __half2float(__half(__nv_cvt_fp8_to_halfraw(vp[c0 + x], __NV_E4M3))) * s;
                 } else {
                   const float y = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(vp)[c0 + x]);
                   if (!(fabsf(y) < INFINITY)) v[x] += y;
@@ -783,6 +787,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (j >= 2 && !warp_wait(v_empty + vs, (j / 2 + 1) & 1, p.status, kTimeoutTmemEmpty, abort)) break;
           const int slot = j % kSlots;
           float* sk = scales + slot * 2 * kTile;
+          // (Not even a weight of zero may meet an appended row's scale that is not finite.)
+          if (kb + i >= seg.cached && !(fabsf(vs_) < INFINITY)) {
+            vs_ = 0.f;
+            odd = true;
+          }
           const uint32_t mine = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs_, 0.f)));
           sk[i] = ks;
           sk[kTile + i] = vs_;

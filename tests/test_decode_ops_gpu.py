@@ -937,3 +937,28 @@ def test_a_row_whose_only_key_is_nan(n, quantized):
         out = ops.paged_tree(q.to(DEV), cache, table, segs, hk, n, n, mask=_pack(ms), keys_per_split=split).cpu()
         _check()
         assert out[2].isnan().all() and ((out.double() - ref).abs() <= tol)[other].all()
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("n", [6, 20, 70])
+def test_scales_that_are_not_finite_stay_with_the_rows_that_see_them(n, bad):
+    ops = _ops()
+    gen = torch.Generator().manual_seed(n)
+    hq, hk, d = 8, 2, 128
+    cache, table, segs, values, tab, sl = _paged([n], [37], hk, d, True, gen)
+    for which, node in ((0, 2), (1, 4)):  # node 2's key, node 4's values
+        b, o = tab[(37 + node) // 16], (37 + node) % 16
+        cache.pages[b, which, :, 16 * d + 4 * o:16 * d + 4 * o + 4] = torch.tensor([bad]).view(torch.uint8).to(DEV)
+    ms = [torch.eye(n, dtype=torch.bool)]
+    ms[0][1, 2] = ms[0][3, 4] = ms[0][n - 1, 0] = True  # row 1 sees the key, row 3 the values
+    q = torch.randn(n, hq, d, generator=gen).to(BF16)
+    ref, weight, err = _attend64(q, values, tab, sl, d ** -0.5, mask=ms)
+    tol = _tolerance(ref, weight, err, d, True)
+    clean = [r for r in range(n) if r not in (1, 2, 3, 4)]
+    for split in (None, 16, 128):
+        out = ops.paged_tree(q.to(DEV), cache, table, segs, hk, n + 37, n, mask=_pack(ms), keys_per_split=split).cpu()
+        _check()
+        assert ((out.double() - ref).abs() <= tol)[clean].all(), split
+        assert not out[[3, 4]].isfinite().any(), split
+        if bad != bad:
+            assert out[1:5].isnan().all(), split
