@@ -114,10 +114,19 @@ void heads(const View& t, const char* name) {
   if (t.ptr % 16 != 0) refuse(n + " must be 16-byte aligned");
 }
 
-// The layer's pages: quantized ones (already checked by their class) when head_dim > 0.
+// Quantized pages of heads of d. (A QuantizedCache checks them too when it is made, but its fields can
+// be set to other ones later.)
+void quantized_pages(const View& t, long d) {
+  if ((d != 64 && d != 128) || t.dtype != at::kByte || t.dim != 4 || t.size[1] != 2 ||
+      t.size[3] != foa::quantized_page_bytes((int)d) || !t.contiguous() || t.ptr % 16 != 0)
+    refuse("quantized pages must be contiguous uint8 [blocks, 2, kv_heads, 16 * head_dim + 64] for a head_dim of 64 or 128, 16-byte aligned");
+}
+
+// The layer's pages: quantized ones when head_dim > 0.
 void pages(const View& t, int quantized_dim, long kv_heads, long d, const char* what) {
   if (quantized_dim > 0) {
-    if (quantized_dim != d || t.dim != 4 || t.size[2] != kv_heads) refuse("the cache has other heads");
+    quantized_pages(t, quantized_dim);
+    if (quantized_dim != d || t.size[2] != kv_heads) refuse("the cache has other heads");
   } else if (t.dtype != at::kBFloat16 || t.dim != 5 || t.size[1] != 2 || t.size[2] != kv_heads || t.size[3] != 16 ||
              t.size[4] != d || !t.contiguous() || t.ptr % 16 != 0) {
     refuse(what);
@@ -284,13 +293,15 @@ py::object tree_attention(py::handle q, py::handle cache, int quantized_dim, py:
   return o;
 }
 
-// Views of quantized pages (checked by their class): the rows' codes, and their scales.
+// Views of quantized pages: the rows' codes, and their scales.
 py::object codes(py::handle pages, long d) {
+  quantized_pages(View(pages, "pages"), d);
   const at::Tensor& x = THPVariable_Unpack(pages.ptr());
   const int64_t page = x.size(3), heads = x.size(2) * page;
   return wrap(x.as_strided({x.size(0), 2, x.size(2), 16, d}, {2 * heads, heads, page, d, 1}));
 }
 py::object scales(py::handle pages, long d) {
+  quantized_pages(View(pages, "pages"), d);
   const at::Tensor& x = THPVariable_Unpack(pages.ptr());
   return wrap(x.slice(3, 16 * d).view(at::kFloat));
 }

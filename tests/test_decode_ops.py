@@ -145,3 +145,41 @@ def test_store_refusals(change, match):
 def test_process_logits_refusals(change, match):
     with pytest.raises(ValueError, match=match):
         ops.process_logits(**{**dict(logits=torch.zeros(2, 10)), **change})
+
+
+def _changed_cache(change):
+    """A QuantizedCache of 4 blocks, 2 heads of 64, changed after its checks."""
+    c = ops.QuantizedCache.empty(4, 2, 64, device="cpu")
+    for name, value in change.items():
+        setattr(c, name, value(c.pages) if callable(value) else value)
+    return c
+
+
+@pytest.mark.parametrize("change", [
+    dict(head_dim=128),
+    dict(head_dim=32),
+    dict(pages=lambda p: p[..., :16 * 64]),                                 # without scales, and with holes
+    dict(pages=lambda p: torch.zeros(4, 2, 2, 16 * 64, dtype=torch.uint8)),
+    dict(pages=lambda p: torch.zeros(4, 1, 2, 16 * 64 + 64, dtype=torch.uint8)),
+    dict(pages=lambda p: torch.zeros(4, 2, 4, 16 * 64 + 64, dtype=torch.uint8)[:, :, ::2]),
+    dict(pages=lambda p: torch.zeros(4, 2, 2, 16 * 64 + 64, dtype=BF16)),
+    dict(pages=lambda p: p[0]),
+    dict(pages=lambda p: torch.zeros(4 * 2 * 2 * 1088 + 8, dtype=torch.uint8)[8:].view(4, 2, 2, 1088)),
+    dict(pages=lambda p: None),
+])
+def test_a_quantized_cache_changed_after_its_checks_is_refused(change):
+    c = _changed_cache(change)
+    for use in (lambda: c.codes, lambda: c.scales,
+                lambda: ops.paged_tree(**{**_tree_args(), "cache": c}),
+                lambda: ops.paged_tree(**{**_tree_args(d=128), "cache": c}),
+                lambda: ops.qk_norm_rope_cache(**{**_store_args(), "cache": c})):
+        with pytest.raises((ValueError, TypeError), match="page|torch tensor"):
+            use()
+
+
+def test_a_quantized_cache_of_other_heads_than_the_rows_is_refused():
+    c = ops.QuantizedCache.empty(4, 2, 64, device="cpu")
+    with pytest.raises(ValueError, match="other heads"):
+        ops.paged_tree(**{**_tree_args(d=128), "cache": c})
+    with pytest.raises(ValueError, match="other heads"):
+        ops.qk_norm_rope_cache(**{**_store_args(d=128), "cache": c})
