@@ -45,6 +45,10 @@ class Scratch:
         self.counters = torch.zeros(counters, dtype=torch.int32, device=device)
         self.status = torch.zeros(4, dtype=torch.int32, device=device)
         self.status_ptr = self.status.data_ptr()
+        # The zeros are there before a kernel of any stream counts or records a status.
+        with torch.cuda.device(device):
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream().synchronize()
 
     def check(self) -> None:
         """Raises RuntimeError when a kernel recorded a failure since the last check."""
@@ -55,6 +59,7 @@ class Scratch:
 
 
 _scratch: dict[int, Scratch] = {}
+_scratch_lock = threading.Lock()
 
 
 def scratch(device: torch.device | None = None) -> Scratch:
@@ -62,5 +67,9 @@ def scratch(device: torch.device | None = None) -> Scratch:
     index = device.index if device.index is not None else torch.cuda.current_device()
     s = _scratch.get(index)
     if s is None:
-        s = _scratch[index] = Scratch(torch.device("cuda", index))
+        # One for all threads, and published for good: kernels keep the status word's address.
+        with _scratch_lock:
+            s = _scratch.get(index)
+            if s is None:
+                s = _scratch[index] = Scratch(torch.device("cuda", index))
     return s

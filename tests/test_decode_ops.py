@@ -183,3 +183,35 @@ def test_a_quantized_cache_of_other_heads_than_the_rows_is_refused():
         ops.paged_tree(**{**_tree_args(d=128), "cache": c})
     with pytest.raises(ValueError, match="other heads"):
         ops.qk_norm_rope_cache(**{**_store_args(d=128), "cache": c})
+
+
+def test_first_calls_at_once_share_one_scratch(monkeypatch):
+    """Kernels keep the address of a device's status word: no second one takes its place."""
+    import importlib
+    import threading
+    import time
+
+    native = importlib.import_module("furiosa_opt_models_b200.ops.native")
+    made = []
+
+    class Slow:
+        def __init__(self, device):
+            time.sleep(0.05)  # as an allocation may, with the interpreter released
+            self.device = device
+            made.append(self)
+
+    monkeypatch.setattr(native, "Scratch", Slow)
+    monkeypatch.setattr(native, "_scratch", {})
+    start, got = threading.Barrier(8), []
+
+    def call(i):
+        start.wait()
+        got.append(native.scratch(torch.device("cuda", i % 2)))
+
+    threads = [threading.Thread(target=call, args=(i,)) for i in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(made) == 2 and len(got) == 8
+    assert all(s is native.scratch(s.device) for s in got)

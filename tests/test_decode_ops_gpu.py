@@ -962,3 +962,27 @@ def test_scales_that_are_not_finite_stay_with_the_rows_that_see_them(n, bad):
         assert not out[[3, 4]].isfinite().any(), split
         if bad != bad:
             assert out[1:5].isnan().all(), split
+
+
+def test_a_status_of_another_stream_outlives_the_first_call(monkeypatch):
+    """The first call's stream is busy when its status word is laid out; a kernel of another stream
+    records a status at once, and nothing erases it."""
+    import importlib
+
+    ops = _ops()
+    fresh = {}
+    for module in ("decode", "native"):
+        monkeypatch.setattr(importlib.import_module("furiosa_opt_models_b200.ops." + module), "_scratch", fresh)
+    x = torch.zeros(1, 64, device=DEV)
+    tokens, starts = torch.zeros(1, dtype=I32, device=DEV), torch.tensor([0, 9], dtype=I32, device=DEV)  # past the list
+    big = torch.randn(4096, 4096, device=DEV)
+    torch.cuda.synchronize()
+    busy, other = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(busy):
+        for _ in range(200):
+            big = (big @ big).tanh()
+        ops.scratch(torch.device("cuda", 0))
+    with torch.cuda.stream(other):
+        ops.process_logits(x, output=(tokens, starts), presence=torch.ones(1, device=DEV))
+    torch.cuda.synchronize()
+    assert int(fresh[0].status[0].item()) == 7
