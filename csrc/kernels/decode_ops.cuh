@@ -72,6 +72,8 @@ struct TreeAttention {
   int* status = nullptr;
 };
 int tree_attention(const TreeAttention& args, cudaStream_t stream);
+// What the grids are laid out for: max_len may be a bound far above any segment that fits the rows.
+inline int longest_segment(const TreeAttention& args) { return args.max_len < args.rows ? args.max_len : args.rows; }
 // The split width that tree_attention works best with for these sizes.
 int tree_attention_split(int num_segments, int q_heads, int kv_heads, int head_dim, int quantized, int max_keys,
                          int max_len);

@@ -615,13 +615,13 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, kQ, NT>::kCtas)
 // keys and 16 heads in 256 splits took 77 us, with sixteen 60. How many take part follows from the
 // row's own splits, so that the order of its sums is the same in every call.
 template <int D, int W>
-__global__ void __launch_bounds__(32 * W) tree_merge_kernel(const TreeAttention p, int max_splits, bool even) {
+__global__ void __launch_bounds__(32 * W) tree_merge_kernel(const TreeAttention p, int max_splits, int longest, bool even) {
   constexpr int E = D / 32;
   __shared__ float sm_acc[W - 1][D], sm_den[W - 1];
   pdl_wait();
   pdl_trigger();
-  const Segment seg = p.segments[blockIdx.x / p.max_len];
-  const int tok = blockIdx.x % p.max_len;
+  const Segment seg = p.segments[blockIdx.x / longest];
+  const int tok = blockIdx.x % longest;
   const int head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (tok >= seg.len || !rows_fit(p, seg) || !segment_fits(p, seg)) return;
   const int nsplit = Parts(seg.cached + seg.len, p.keys_per_split, even).count;
@@ -686,9 +686,10 @@ __global__ void __launch_bounds__(32 * W) tree_merge_kernel(const TreeAttention 
 template <int D>
 int merge(const TreeAttention& p, int splits, bool even, cudaStream_t stream) {
   if (splits == 1) return 0;
-  const dim3 grid(p.num_segments * p.max_len, p.q_heads);
-  const cudaError_t rc = splits > 16 ? launch_pdl(tree_merge_kernel<D, 16>, grid, dim3(512), 0, stream, p, splits, even)
-                                     : launch_pdl(tree_merge_kernel<D, 4>, grid, dim3(128), 0, stream, p, splits, even);
+  const int longest = longest_segment(p);
+  const dim3 grid(p.num_segments * longest, p.q_heads);
+  const cudaError_t rc = splits > 16 ? launch_pdl(tree_merge_kernel<D, 16>, grid, dim3(512), 0, stream, p, splits, longest, even)
+                                     : launch_pdl(tree_merge_kernel<D, 4>, grid, dim3(128), 0, stream, p, splits, longest, even);
   return rc == cudaSuccess ? 0 : -5;
 }
 
@@ -696,7 +697,7 @@ template <int D, bool kQ, int NT>
 int launch(const TreeAttention& p, cudaStream_t stream) {
   const int G = p.q_heads / p.kv_heads;
   const int splits = ((long)p.max_keys + p.keys_per_split - 1) / p.keys_per_split;
-  const long mtiles = ((long)p.max_len * G + 8 * NT - 1) / (8 * NT);
+  const long mtiles = ((long)longest_segment(p) * G + 8 * NT - 1) / (8 * NT);
   const long ctas = mtiles * p.kv_heads * p.num_segments;
   if (ctas > 2147483647L) return -2;
   constexpr int smem = Shape<D, kQ, NT>::kSmem;
@@ -757,7 +758,7 @@ int tree_attention(const TreeAttention& p, cudaStream_t stream) {
   if (p.num_segments <= 0 || p.rows <= 0) return 0;
   if (p.kv_heads <= 0 || p.q_heads <= 0 || p.q_heads % p.kv_heads != 0) return -2;
   if (p.max_keys <= 0 || p.max_len <= 0 || p.keys_per_split <= 0 || p.keys_per_split % 16 != 0) return -2;
-  if ((long)p.num_segments * p.max_len > 2147483647L || p.q_heads > 65535) return -2;
+  if ((long)p.num_segments * longest_segment(p) > 2147483647L || p.q_heads > 65535) return -2;
   const long splits = ((long)p.max_keys + p.keys_per_split - 1) / p.keys_per_split;
   if (splits > 65535) return -2;
   if (splits > 1 && (p.partial_o == nullptr || p.partial_ml == nullptr ||

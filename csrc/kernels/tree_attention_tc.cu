@@ -902,7 +902,7 @@ int launch(const TreeAttention& p, int splits, cudaStream_t stream) {
   using C = Cfg<D, kQ>;
   static_assert(C::kSmem <= 232448, "shared memory");
   const int G = p.q_heads / p.kv_heads;
-  const long mtiles = ((long)p.max_len * G + 2 * kTile - 1) / (2 * kTile);
+  const long mtiles = ((long)longest_segment(p) * G + 2 * kTile - 1) / (2 * kTile);
   const long ctas = mtiles * p.kv_heads * p.num_segments;
   if (ctas > 2147483647L) return -2;
   const long pages = p.cache_blocks * 2 * p.kv_heads;

@@ -986,3 +986,24 @@ def test_a_status_of_another_stream_outlives_the_first_call(monkeypatch):
         ops.process_logits(x, output=(tokens, starts), presence=torch.ones(1, device=DEV))
     torch.cuda.synchronize()
     assert int(fresh[0].status[0].item()) == 7
+
+
+@pytest.mark.parametrize("quantized", [True, False], ids=["e4m3", "bf16"])
+def test_bounds_far_above_the_lengths(quantized):
+    """max_len and max_keys at their largest, as a captured call may give them, and many empty segments:
+    what is launched follows the rows that exist."""
+    ops = _ops()
+    gen = torch.Generator().manual_seed(1)
+    hq, hk, d = 8, 2, 64
+    lens, cached = [1, 3, 2], [40, 90, 7]
+    cache, table, segs, values, tab, sl = _paged(lens, cached, hk, d, quantized, gen)
+    many = torch.zeros(300, 5, dtype=I32, device=DEV)
+    many[[0, 150, 299]] = segs
+    q = torch.randn(6, hq, d, generator=gen).to(BF16)
+    ref, weight, err = _attend64(q, values, tab, sl, d ** -0.5)
+    tol = _tolerance(ref, weight, err, d, quantized)
+    for split in (None, 64, 1 << 20):
+        keys = 1 << 30 if split is None or split > 64 else 128
+        out = ops.paged_tree(q.to(DEV), cache, table, many, hk, keys, 1 << 24, keys_per_split=split)
+        _check()
+        assert ((out.double().cpu() - ref).abs() <= tol).all()
