@@ -3,17 +3,22 @@
 // costs its set-up). A row's parts follow from its own keys and the given width alone.
 #pragma once
 
+#ifdef __CUDACC__
+#define FOA_HOST_DEVICE __host__ __device__ __forceinline__
+#else
+#define FOA_HOST_DEVICE inline
+#endif
+
 namespace foa {
 
 struct Parts {
   int width, count;  // keys of a part (at most the given width), parts
-  __device__ __forceinline__ Parts(int keys, int keys_per_split, bool even) : width(keys_per_split) {
-    count = (keys + keys_per_split - 1) / keys_per_split;
-    if (!even || count == 1 || keys_per_split % 128 != 0 || keys >= 1 << 22) return;
-    // At least keys / count, rounded up to tiles (the quotient is off by less than one).
-    width = ((int)__fdividef((float)keys, (float)count) + 128) / 128 * 128;
-    if (width > keys_per_split) width = keys_per_split;
-    while ((count - 1) * width >= keys) --count;
+  FOA_HOST_DEVICE Parts(int keys, int keys_per_split, bool even)
+      : width(keys_per_split), count((keys + keys_per_split - 1) / keys_per_split) {
+    if (!even || count == 1 || keys_per_split % 128 != 0) return;
+    const int tiles = (keys + 127) / 128, each = (tiles + count - 1) / count;
+    width = 128 * each;
+    count = (tiles + each - 1) / each;
   }
 };
 

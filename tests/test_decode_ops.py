@@ -215,3 +215,26 @@ def test_first_calls_at_once_share_one_scratch(monkeypatch):
         t.join()
     assert len(made) == 2 and len(got) == 8
     assert all(s is native.scratch(s.device) for s in got)
+
+
+def _parts(keys, width, even):
+    from furiosa_opt_models_b200.ops.native import native
+
+    return native().ops.history_parts(keys, width, even)
+
+
+def test_parts_of_a_history_are_equal_in_whole_tiles():
+    # Eight parts of 1024 keys, not seven of 1152 and one of 128.
+    assert _parts(8192, 1152, True) == (1024, 8)
+    assert _parts(4096, 1152, True) == (1024, 4) and _parts(768, 512, True) == (384, 2)
+    for keys in [*range(1, 3000), 8191, 8192, 8193, 131072, (1 << 22) - 1, 1 << 22, (1 << 22) + 129, (1 << 30) - 5, 1 << 30]:
+        for width in (128, 256, 384, 1152, 4096, 1 << 20):
+            each, count = _parts(keys, width, True)
+            least = -(-keys // width)  # as few parts as the width allows, or fewer where whole tiles do it
+            assert each <= width and (each % 128 == 0 or count == 1) and 1 <= count <= least
+            assert (count - 1) * each < keys <= count * each
+            if count > 1:
+                assert (each - 128) * least < keys  # one tile less would not do
+    for keys, width in ((1, 16), (17, 16), (1000, 48), (129, 128), (1 << 30, 1 << 30)):
+        assert _parts(keys, width, False) == (width, -(-keys // width))
+        assert _parts(keys, 48, True) == (48, -(-keys // 48))  # no whole tiles: parts as given
