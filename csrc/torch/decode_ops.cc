@@ -133,6 +133,17 @@ void pages(const View& t, int quantized_dim, long kv_heads, long d, const char* 
   }
 }
 
+// Two tensors of as many rows of `width` bytes (elements of `size` bytes) are the same one or share
+// nothing: rows are read while others are written.
+void same_or_apart(const View& a, const View& b, long width, long size, const char* what) {
+  const long rows = a.size[0], as = rows > 1 ? a.stride[0] * size : width, bs = rows > 1 ? b.stride[0] * size : width;
+  if (rows == 0 || (a.ptr == b.ptr && as == bs)) return;
+  if (a.ptr + (rows - 1) * as + width <= b.ptr || b.ptr + (rows - 1) * bs + width <= a.ptr) return;
+  // Side by side in the rows of one tensor.
+  const long shift = (((long)(b.ptr - a.ptr)) % as + as) % as;
+  if (as != bs || shift < width || shift + width > as) refuse(what);
+}
+
 template <class T>
 T* at(uint64_t p) {
   return reinterpret_cast<T*>(p);
@@ -239,6 +250,7 @@ py::object tree_attention(py::handle q, py::handle cache, int quantized_dim, py:
     const View y(out, "out");
     heads(y, "out");
     if (!y.is({rows, q_heads, d})) refuse("out must have the shape of q");
+    same_or_apart(x, y, q_heads * d * 2, 2, "out must be q itself or not overlap it");
     place.with(y);
     o = py::reinterpret_borrow<py::object>(out);
     a.o = at<__nv_bfloat16>(y.ptr);
@@ -374,6 +386,8 @@ py::object process_logits(py::handle logits, py::handle prompt, py::handle outpu
     const View v(out, "out");
     if (v.dtype != x.dtype || !v.is({rows, vocab}) || (v.stride[1] != 1 && vocab != 1) || (rows > 1 && v.stride[0] < vocab))
       refuse("out must have the logits' shape and type, and unit column stride");
+    const long size = x.dtype == at::kFloat ? 4 : 2;
+    same_or_apart(x, v, vocab * size, size, "out must be the logits themselves or not overlap them");
     place.with(v);
     a.out = at<void>(v.ptr);
     a.ldo = v.stride[0];

@@ -112,7 +112,8 @@ def paged_tree(q, cache, table, segments, kv_heads, max_keys, max_len, mask=None
     (positions below ``cached``) and the appended rows j whose bit j is set in its words of ``mask``
     (int32 [rows, words], bit j % 32 of word j / 32: ``tree_mask`` makes it from drafted trees); with
     ``mask=None`` the rows j <= i, as in a chain of drafts or a prompt chunk. A row that sees nothing
-    gets zeros; a row of q with an element that is not finite gets NaN from any key it sees. Rows of ``out`` that belong to no segment are left as they were.
+    gets zeros; a row of q with an element that is not finite gets NaN from any key it sees. ``out`` is
+    q itself or memory apart from it; its rows that belong to no segment are left as they were.
 
     ``max_keys`` bounds every segment's cached + len and ``max_len`` its len: a segment that goes
     past one of them (or past its table or the rows) gets zeros and records a status. A history is
@@ -139,7 +140,7 @@ def process_logits(logits, prompt=None, output=None, repetition=None, frequency=
     - bit t % 32 of word t / 32 of the row of ``allowed`` (int32 [rows, words]) unset: -inf.
 
     ``repetition``, ``frequency`` and ``presence`` are FP32 [rows]. ``out`` (the logits' shape and
-    type; may be ``logits``) receives the adjusted logits. A logit that is NaN is never chosen; a row
-    whose every token is -inf (or NaN) gives index -1 and value -inf."""
+    type; ``logits`` itself, or memory apart from them) receives the adjusted logits. A logit that is
+    NaN is never chosen; a row whose every token is -inf (or NaN) gives index -1 and value -inf."""
     return calls().process_logits(logits, prompt, output, repetition, frequency, presence, bias, allowed, out,
                                   _status(logits))

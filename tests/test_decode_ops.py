@@ -238,3 +238,42 @@ def test_parts_of_a_history_are_equal_in_whole_tiles():
     for keys, width in ((1, 16), (17, 16), (1000, 48), (129, 128), (1 << 30, 1 << 30)):
         assert _parts(keys, width, False) == (width, -(-keys // width))
         assert _parts(keys, 48, True) == (48, -(-keys // 48))  # no whole tiles: parts as given
+
+
+@pytest.mark.parametrize("rows,of,out,fine", [
+    (3, (0, 4 * 64), (0, 4 * 64), True),                # q itself
+    (3, (0, 4 * 64), (3 * 4 * 64, 4 * 64), True),       # behind it
+    (3, (0, 8 * 64), (4 * 64, 8 * 64), True),           # beside it, in the same rows
+    (3, (4 * 64, 8 * 64), (0, 8 * 64), True),
+    (1, (0, 8 * 64), (0, 4 * 64), True),                # one row: its stride says nothing
+    (3, (0, 4 * 64), (4 * 64, 4 * 64), False),          # a row further
+    (3, (0, 8 * 64), (2 * 64, 8 * 64), False),          # two heads further
+    (3, (0, 8 * 64), (6 * 64, 8 * 64), False),          # into the next row
+    (3, (0, 4 * 64), (0, 8 * 64), False),               # other strides
+    (1, (0, 4 * 64), (8, 4 * 64), False),
+])
+def test_out_that_overlaps_q_is_refused(rows, of, out, fine):
+    mem = torch.zeros(4096, dtype=BF16)
+    view = lambda v: mem.as_strided((rows, 4, 64), (v[1], 64, 1), v[0])  # noqa: E731
+    with pytest.raises(ValueError, match="CUDA" if fine else "overlap"):
+        ops.paged_tree(**{**_tree_args(rows=rows), "q": view(of), "out": view(out)})
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,of,out,fine", [
+    (3, (0, 10), (0, 10), True),
+    (3, (0, 10), (30, 10), True),
+    (3, (0, 25), (10, 25), True),
+    (3, (15, 25), (0, 25), True),
+    (1, (0, 25), (0, 10), True),
+    (3, (0, 10), (10, 10), False),
+    (3, (0, 10), (1, 10), False),
+    (3, (1, 10), (0, 10), False),
+    (3, (0, 25), (20, 25), False),
+    (3, (0, 20), (0, 10), False),
+])
+def test_out_that_overlaps_the_logits_is_refused(rows, of, out, fine, dtype):
+    mem = torch.zeros(200, dtype=dtype)
+    view = lambda v: mem.as_strided((rows, 10), (v[1], 1), v[0])  # noqa: E731
+    with pytest.raises(ValueError, match="CUDA" if fine else "overlap"):
+        ops.process_logits(view(of), out=view(out))

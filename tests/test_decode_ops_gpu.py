@@ -1007,3 +1007,28 @@ def test_bounds_far_above_the_lengths(quantized):
         out = ops.paged_tree(q.to(DEV), cache, table, many, hk, keys, 1 << 24, keys_per_split=split)
         _check()
         assert ((out.double().cpu() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("quantized", [True, False], ids=["e4m3", "bf16"])
+@pytest.mark.parametrize("n", [1, 6, 20, 70])
+def test_attention_written_over_its_queries(n, quantized):
+    ops = _ops()
+    gen = torch.Generator().manual_seed(n)
+    hq, hk, d = 8, 2, 128
+    lens, cached = [n, (n + 1) // 2, n], [700, 30, 0]
+    cache, table, segs, _, _, _ = _paged(lens, cached, hk, d, quantized, gen)
+    q = torch.randn(sum(lens) + 1, hq, d, generator=gen).to(BF16).to(DEV)
+    for split in (None, 128, 4096):
+        want = q.clone()
+        ops.paged_tree(q, cache, table, segs, hk, 700 + n, n, keys_per_split=split, out=want)
+        for _ in range(5):
+            got = q.clone()
+            ops.paged_tree(got, cache, table, segs, hk, 700 + n, n, keys_per_split=split, out=got)
+            assert torch.equal(got, want)
+    # Beside the queries, in the rows of one tensor.
+    both = torch.cat([q, torch.zeros_like(q)], 1)
+    ops.paged_tree(both[:, :hq], cache, table, segs, hk, 700 + n, n, keys_per_split=128, out=both[:, hq:])
+    apart = torch.zeros_like(q)
+    ops.paged_tree(q, cache, table, segs, hk, 700 + n, n, keys_per_split=128, out=apart)
+    _check()
+    assert torch.equal(both[:, :hq], q) and torch.equal(both[:, hq:], apart)
