@@ -10,6 +10,7 @@
 #include <pybind11/pybind11.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
@@ -257,6 +258,7 @@ py::object tree_attention(py::handle q, py::handle cache, int quantized_dim, py:
     a.ld_o = rows > 1 ? y.stride[0] : q_heads * d;
   }
   const float s = scale.is_none() ? (d == 64 ? 0.125f : 0.08838834764831845f) : py::cast<float>(scale);
+  if (!std::isfinite(s)) refuse("scale must be finite in FP32");
   place.check();
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)place.device);
   if (out.is_none()) {

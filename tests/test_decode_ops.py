@@ -277,3 +277,9 @@ def test_out_that_overlaps_the_logits_is_refused(rows, of, out, fine, dtype):
     view = lambda v: mem.as_strided((rows, 10), (v[1], 1), v[0])  # noqa: E731
     with pytest.raises(ValueError, match="CUDA" if fine else "overlap"):
         ops.process_logits(view(of), out=view(out))
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 1e39])
+def test_a_scale_that_is_not_finite_is_refused(scale):
+    with pytest.raises(ValueError, match="scale must be finite"):
+        ops.paged_tree(**_tree_args(), scale=scale)
