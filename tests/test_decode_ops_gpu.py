@@ -1032,3 +1032,142 @@ def test_attention_written_over_its_queries(n, quantized):
     ops.paged_tree(q, cache, table, segs, hk, 700 + n, n, keys_per_split=128, out=apart)
     _check()
     assert torch.equal(both[:, :hq], q) and torch.equal(both[:, hq:], apart)
+
+
+@pytest.mark.parametrize("quantized", [True, False], ids=["e4m3", "bf16"])
+@pytest.mark.parametrize("n", [1, 6, 20, 70])
+def test_a_negative_scale(n, quantized):
+    ops = _ops()
+    gen = torch.Generator().manual_seed(n)
+    hq, hk, d = 8, 2, 64
+    cache, table, segs, values, tab, sl = _paged([n], [200], hk, d, quantized, gen)
+    q = torch.randn(n, hq, d, generator=gen).to(BF16)
+    ref, weight, err = _attend64(q, values, tab, sl, -0.3)
+    tol = _tolerance(ref, weight, tuple(e.abs() for e in _attend64(q, values, tab, sl, 0.3)[2]), d, quantized)
+    for split in (None, 16, 128):
+        out = ops.paged_tree(q.to(DEV), cache, table, segs, hk, n + 200, n, scale=-0.3, keys_per_split=split)
+        _check()
+        assert ((out.double().cpu() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("tied", [
+    [4, 5, 7], [13, 1024 + 8, 3], [2048 + 7, 2048 + 5], [8191, 9000, 20000], [20000, 16384], [0, 24999], [24999],
+    [24998, 24999], list(range(25000)),
+])
+@pytest.mark.parametrize("pad", [0, 1, 5])
+def test_the_first_of_equal_maxima_is_chosen(tied, pad, dtype):
+    """Equal maxima inside a vector, across a thread's vectors, in a row's unaligned ends and in other
+    slices, among values that are below them; with a list, a listed token may be one of them."""
+    ops = _ops()
+    vocab = 25000
+    wide = torch.full((3, vocab + pad), -1.0, dtype=dtype, device=DEV)
+    x = wide[:, pad:]
+    x[:, tied] = 2.5
+    index, value = ops.process_logits(x)
+    assert index.tolist() == [min(tied)] * 3 and value.tolist() == [2.5] * 3
+    # A listed token that ends at the same value, before and behind the others (3.5 - 1 = 2.5).
+    for token in (1, 8190, vocab - 2):
+        x[:, tied] = 2.5
+        x[:, token] = 3.5
+        lists = (torch.tensor([token], dtype=I32, device=DEV), torch.tensor([0, 1, 1, 1], dtype=I32, device=DEV))
+        index, value = ops.process_logits(x, output=lists, presence=torch.ones(3, device=DEV))
+        assert index.tolist() == [min([token] + tied), token, token] and value.tolist() == [2.5, 3.5, 3.5]
+        x[:, token] = -1.0
+    # The first is not allowed: the next one.
+    if len(tied) > 1:
+        x[:, tied] = 2.5
+        allowed = torch.ones(3, vocab, dtype=torch.bool)
+        allowed[1, min(tied)] = False
+        index, _ = ops.process_logits(x, allowed=_bits(allowed))
+        assert index.tolist() == [min(tied), sorted(tied)[1], min(tied)]
+    _check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_infinite_logits(dtype):
+    ops = _ops()
+    inf = float("inf")
+    x = torch.randn(4, 9001, device=DEV).to(dtype)
+    x[0, 8500] = x[0, 77] = inf
+    x[1] = -inf
+    x[2] = float("nan")
+    x[3, :9000] = -inf
+    one = lambda t: (torch.tensor([t], dtype=I32, device=DEV), torch.tensor([0, 1, 1, 1, 1], dtype=I32, device=DEV))  # noqa: E731
+    for kw in ({}, dict(output=one(77), frequency=torch.ones(4, device=DEV))):
+        out = torch.empty_like(x)
+        index, value = ops.process_logits(x, out=out, **kw)
+        assert index.tolist() == [77, -1, -1, 9000]
+        assert value.tolist()[:3] == [inf, -inf, -inf] and value[3] == x[3, 9000]
+        assert torch.equal(out.nan_to_num(5.0), x.nan_to_num(5.0))
+    index, value = ops.process_logits(x, prompt=one(77), repetition=torch.full((4,), inf, device=DEV))
+    assert index[0] == 8500 and value[0] == inf  # inf / inf is NaN and never chosen
+    _check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [33, 20011])
+def test_masks_that_are_wide_strided_or_shared(vocab, dtype):
+    ops = _ops()
+    gen = torch.Generator().manual_seed(vocab)
+    x = torch.randn(5, vocab, generator=gen).to(dtype).to(DEV)
+    allowed = torch.rand(5, vocab, generator=gen) < 0.3
+    bits = _bits(allowed)
+    words = bits.shape[1]
+    want, best = torch.empty_like(x), x.masked_fill(~allowed.to(DEV), -torch.inf)
+    i0, v0 = ops.process_logits(x, allowed=bits, out=want)
+    assert torch.equal(want, best) and torch.equal(v0, best.float().amax(1))
+    for extra, skip in ((1, 0), (7, 3), (64, 1)):  # wider than it must be, rows of a wider tensor
+        wide = torch.full((5, skip + words + extra), -1, dtype=I32, device=DEV)
+        wide[:, skip:skip + words] = bits
+        for view in (wide[:, skip:], wide[:, skip:skip + words]):
+            out = torch.empty_like(x)
+            i, v = ops.process_logits(x, allowed=view, out=out)
+            assert torch.equal(i, i0) and torch.equal(v, v0) and torch.equal(out, want)
+    shared = bits[1:2].expand(5, words)  # one mask for every row
+    _, v = ops.process_logits(x, allowed=shared)
+    assert torch.equal(v, x.masked_fill(~allowed[1].to(DEV), -torch.inf).float().amax(1))
+    _check()
+
+
+def test_calls_from_several_threads():
+    """The calls release the interpreter: four threads on streams of their own, each with its inputs."""
+    import threading
+
+    ops = _ops()
+    hq, hk, d = 8, 2, 64
+    jobs = []
+    for i in range(4):
+        gen = torch.Generator().manual_seed(i)
+        n = (1, 5, 20, 40)[i]
+        cache, table, segs, _, _, _ = _paged([n] * 3, [100, 900, 40], hk, d, True, gen)
+        q = torch.randn(3 * n, hq, d, generator=gen).to(BF16).to(DEV)
+        x = torch.randn(4, 30000 + i, generator=gen).to(DEV)
+        jobs.append((q, cache, table, segs, n, x))
+
+    def call(job):
+        q, cache, table, segs, n, x = job
+        return (ops.paged_tree(q, cache, table, segs, hk, 900 + n, n, keys_per_split=128),) + ops.process_logits(x)
+
+    want = [call(j) for j in jobs]
+    torch.cuda.synchronize()
+    faults = []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(50):
+                    got = call(jobs[i])
+                    stream.synchronize()
+                    assert all(torch.equal(a, b) for a, b in zip(got, want[i]))
+        except BaseException as e:  # noqa: BLE001
+            faults.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    _check()
+    assert not faults, faults[0]
