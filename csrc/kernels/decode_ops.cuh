@@ -77,7 +77,8 @@ inline int longest_segment(const TreeAttention& args) { return args.max_len < ar
 // The split width that tree_attention works best with for these sizes.
 int tree_attention_split(int num_segments, int q_heads, int kv_heads, int head_dim, int quantized, int max_keys,
                          int max_len);
-// The tcgen05 form, for segments whose rows times group heads fill more than one MMA row tile.
+// The tcgen05 form, for segments of more (token, head) rows a key/value head than 16 (BF16 pages) or 32
+// (codes): 256 rows a CTA, so the fewest fill an eighth of its tiles, and still come out ahead.
 bool tree_attention_tc_supported(const TreeAttention& args);
 int tree_attention_tc(const TreeAttention& args, cudaStream_t stream);
 

@@ -1,6 +1,6 @@
 // Attention of chunks and drafted token trees over the paged cache on the tcgen05 tensor cores, for
-// segments whose (token, head) rows fill an MMA tile; tree_attention.cu states the operator and
-// takes the others.
+// segments of more than 16 (token, head) rows a key/value head, 32 over codes; tree_attention.cu states
+// the operator, the rule and takes the others.
 //
 // One CTA per (segment, key/value head, 256 rows, split of the keys), 128-key tiles:
 // - Two softmax warpgroups, a thread a row, each with its own S and O in TMEM. With more than 128
@@ -20,7 +20,9 @@
 //   largest that the row sees does; O is rescaled in TMEM then, which takes 3000 cycles beside 3700 of a
 //   pair of tiles. With slack 2^4 that happened to a warp in every third tile early on; FP16 weights of
 //   slack 2^8 still hold 2^-20 of the reference in full and 2^-30 at all. Both are part of the unit that
-//   O and the row's sum are held in.
+//   O and the row's sum are held in. So a seen key whose V scale is 2^20 times the others' costs those
+//   bits, however small its weight; and since weights before V's scale are FP32 in units of V's
+//   reference 2^e, those below 2^(e - 132) of the row's largest flush (e > 100: values near BF16's end).
 // - Every wait is bounded; a timeout records a status and every role leaves through the same end.
 //
 // What bounds it: the chain of one warpgroup (128 scores a thread, P to TMEM, P V, the next S, which
