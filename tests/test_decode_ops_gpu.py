@@ -1171,3 +1171,44 @@ def test_calls_from_several_threads():
         t.join()
     _check()
     assert not faults, faults[0]
+
+
+def test_captured_calls_of_many_parts_and_slices_replay_side_by_side():
+    """Two graphs of wide trees in several parts and of logits in several slices, on two streams at once."""
+    ops = _ops()
+    gen = torch.Generator().manual_seed(1)
+    hk, vocab = 2, 40000
+    jobs = []
+    for quantized in (True, False):
+        cache, table, segs, _, _, _ = _paged([40, 20, 33], [900, 2000, 5], hk, 128, quantized, gen)
+        q = torch.randn(93, 8, 128, generator=gen).to(BF16).to(DEV)
+        x = torch.randn(93, vocab, generator=gen).to(DEV)
+        lists = (torch.randint(0, vocab, (93 * 50,), generator=gen).to(I32).to(DEV), (torch.arange(94) * 50).to(I32).to(DEV))
+        ones = torch.ones(93, device=DEV)
+
+        def call(q=q, cache=cache, table=table, segs=segs, x=x, lists=lists, ones=ones):
+            o = ops.paged_tree(q, cache, table, segs, hk, 2040, 40, keys_per_split=256)
+            out = torch.empty_like(x)
+            return (o, out) + ops.process_logits(x, output=lists, frequency=ones, out=out)
+
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = call()
+        jobs.append((call, graph, outs, q, x))
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for _ in range(3):
+        for _, _, _, q, x in jobs:
+            q.copy_(torch.randn(q.shape, device=DEV))
+            x.copy_(torch.randn(x.shape, device=DEV))
+        wants = [[t.clone() for t in call()] for call, _, _, _, _ in jobs]
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for (_, graph, _, _, _), stream in zip(jobs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for want, (_, _, outs, _, _) in zip(wants, jobs):
+            assert all(torch.equal(a, b) for a, b in zip(want, outs))
+    _check()
